@@ -1,0 +1,367 @@
+// torch.ops.tdc.* of the row operators (rows_*.hip).  Unlike the iteration's ops, which write
+// into buffers of the engine, these return new tensors: a request is one call from Python,
+// and under graph capture the allocations belong to the graph's own pool.
+#include <torch/extension.h>
+#include <ATen/hip/HIPContext.h>
+#include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
+#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+
+#include <limits>
+
+#include "kernels.h"
+
+namespace {
+
+using at::Tensor;
+using OptTensor = std::optional<Tensor>;
+using DevGuard = at::hip::HIPGuardMasqueradingAsCUDA;
+
+hipStream_t cur_stream() { return at::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream(); }
+
+constexpr int64_t MAX_WIDTH = 16384;
+constexpr int64_t MAX_SLOTS = std::numeric_limits<int32_t>::max() - 1;
+
+int code_of(at::ScalarType t, const char* what) {
+  switch (t) {
+    case at::kFloat: return TDC_F32;
+    case at::kHalf: return TDC_F16;
+    case at::kBFloat16: return TDC_BF16;
+    default: TORCH_CHECK(false, "tdc: ", what, " must be fp32, fp16 or bf16, got ", t);
+  }
+  return -1;
+}
+
+void check(int err, const char* what) {
+  TORCH_CHECK(err == 0, "tdc: ", what, " failed: ", hipGetErrorString((hipError_t)err), " (code ",
+              err, ")");
+}
+
+bool has(const OptTensor& t) { return t.has_value() && t->defined(); }
+
+// Rows on the GPU with neighbouring columns.
+void check_rows(const Tensor& x, const char* name) {
+  TORCH_CHECK(x.is_cuda() && x.dim() == 2 && (x.stride(1) == 1 || x.size(1) <= 1), "tdc: ", name,
+              " must be rows [N, D] on the GPU with contiguous columns");
+}
+
+void check_like(const Tensor& t, const Tensor& x, const char* name) {
+  check_rows(t, name);
+  TORCH_CHECK(t.device() == x.device() && t.scalar_type() == x.scalar_type() && t.sizes() == x.sizes(),
+              "tdc: ", name, " must have the shape, type and device of the rows");
+}
+
+// Weights of `n` elements: null, fp32 (w32) or the rows' type.
+const void* weights_of(const OptTensor& w, const Tensor& x, int64_t n, bool& w32) {
+  w32 = true;
+  if (!has(w)) return nullptr;
+  TORCH_CHECK(w->device() == x.device() && w->is_contiguous() && w->numel() == n,
+              "tdc: weights must be contiguous, on the rows' device and match their shape");
+  w32 = w->scalar_type() == at::kFloat;
+  TORCH_CHECK(w32 || w->scalar_type() == x.scalar_type(),
+              "tdc: weights must be fp32 or of the rows' type");
+  return w->data_ptr();
+}
+
+void check_index(const Tensor& t, const Tensor& x, int64_t n, const char* name) {
+  TORCH_CHECK(t.device() == x.device() && t.scalar_type() == at::kInt && t.is_contiguous() &&
+                  t.numel() == n,
+              "tdc: ", name, " must be int32 [", n, "] on the rows' device");
+}
+
+int num_cus(const Tensor& t) {
+  int v = 0;
+  if (hipDeviceGetAttribute(&v, hipDeviceAttributeMultiprocessorCount, t.device().index()) !=
+          hipSuccess || v <= 0)
+    v = 256;
+  return v;
+}
+
+// ------------------------------------------------------------------ norm
+std::vector<Tensor> rms_norm(const Tensor& x, const OptTensor& w, const OptTensor& r, double eps,
+                             bool want_rstd, int64_t fp8_width) {
+  check_rows(x, "x");
+  const int64_t n = x.size(0), d = x.size(1);
+  const int code = code_of(x.scalar_type(), "x");
+  TORCH_CHECK(d >= 1 && d <= MAX_WIDTH && fp8_width <= MAX_WIDTH, "tdc.rms_norm: 1 to ", MAX_WIDTH,
+              " columns, got ", d);
+  TORCH_CHECK(fp8_width == 0 || (fp8_width % 32 == 0 && fp8_width >= d), "tdc.rms_norm: fp8 width");
+  if (has(r)) check_like(*r, x, "residual");
+  bool w32;
+  const void* wp = weights_of(w, x, d, w32);
+  const DevGuard guard(x.device());
+  std::vector<Tensor> res;
+  Tensor q, s, y;
+  if (fp8_width) {
+    q = at::empty({n, fp8_width}, x.options().dtype(at::kFloat8_e4m3fn));
+    s = at::empty({n, fp8_width / 32}, x.options().dtype(at::kByte));
+    res = {q, s};
+  } else {
+    y = at::empty({n, d}, x.options());
+    res = {y};
+  }
+  Tensor h, rstd;
+  if (has(r)) {
+    h = at::empty({n, d}, x.options());
+    res.push_back(h);
+  }
+  if (want_rstd) {
+    rstd = at::empty({n}, x.options().dtype(at::kFloat));
+    res.push_back(rstd);
+  }
+  check(tdc_rms_norm(code, x.data_ptr(), x.stride(0), has(r) ? r->data_ptr() : nullptr,
+                     has(r) ? r->stride(0) : 0, wp, w32, n, (int)d, (float)eps,
+                     y.defined() ? y.data_ptr() : nullptr, q.defined() ? q.data_ptr() : nullptr,
+                     s.defined() ? s.data_ptr() : nullptr, (int)fp8_width,
+                     h.defined() ? h.data_ptr() : nullptr,
+                     rstd.defined() ? rstd.data_ptr<float>() : nullptr, cur_stream()),
+        "rms_norm");
+  return res;
+}
+
+std::vector<Tensor> rms_norm_bwd(const Tensor& h, const OptTensor& w, const Tensor& rstd,
+                                 const Tensor& dy, const OptTensor& dh, bool want_dw) {
+  check_rows(h, "h");
+  check_like(dy, h, "dy");
+  if (has(dh)) check_like(*dh, h, "dh");
+  const int64_t n = h.size(0), d = h.size(1);
+  const int code = code_of(h.scalar_type(), "h");
+  TORCH_CHECK(d >= 1 && d <= MAX_WIDTH, "tdc.rms_norm_bwd: width");
+  TORCH_CHECK(rstd.device() == h.device() && rstd.scalar_type() == at::kFloat &&
+                  rstd.is_contiguous() && rstd.numel() == n, "tdc.rms_norm_bwd: rstd fp32 [N]");
+  TORCH_CHECK(!want_dw || has(w), "tdc.rms_norm_bwd: dw needs the weights");
+  bool w32;
+  const void* wp = weights_of(w, h, d, w32);
+  const DevGuard guard(h.device());
+  Tensor dx = at::empty({n, d}, h.options());
+  std::vector<Tensor> res = {dx};
+  Tensor part, dw;
+  const int parts = tdc_rms_norm_bwd_parts(n, num_cus(h));
+  if (want_dw) {
+    dw = at::empty({d}, w->options());
+    part = at::empty({parts, d}, h.options().dtype(at::kFloat));
+    res.push_back(dw);
+  }
+  check(tdc_rms_norm_bwd(code, h.data_ptr(), h.stride(0), rstd.data_ptr<float>(), wp, w32,
+                         dy.data_ptr(), dy.stride(0), has(dh) ? dh->data_ptr() : nullptr,
+                         has(dh) ? dh->stride(0) : 0, n, (int)d, dx.data_ptr(),
+                         part.defined() ? part.data_ptr<float>() : nullptr, parts,
+                         dw.defined() ? dw.data_ptr() : nullptr, cur_stream()),
+        "rms_norm_bwd");
+  return res;
+}
+
+Tensor dequant_fp8(const Tensor& q, const Tensor& s, int64_t d, at::ScalarType dtype) {
+  TORCH_CHECK(q.is_cuda() && q.scalar_type() == at::kFloat8_e4m3fn && q.dim() == 2 &&
+                  q.is_contiguous() && q.size(1) % 32 == 0 && d >= 1 && d <= q.size(1) &&
+                  reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0,
+              "tdc.dequant_fp8: q float8_e4m3fn [N, 32 m], 16-byte aligned");
+  TORCH_CHECK(s.device() == q.device() && s.scalar_type() == at::kByte && s.is_contiguous() &&
+                  s.numel() == q.size(0) * (q.size(1) / 32), "tdc.dequant_fp8: s uint8 [N, m]");
+  const int code = code_of(dtype, "dtype");
+  const DevGuard guard(q.device());
+  Tensor out = at::empty({q.size(0), d}, q.options().dtype(dtype));
+  check(tdc_dequant_fp8(code, q.data_ptr(), s.data_ptr(), q.size(0), (int)d, (int)q.size(1),
+                        out.data_ptr(), cur_stream()),
+        "dequant_fp8");
+  return out;
+}
+
+// ------------------------------------------------------------------ gate
+struct MaskArg {
+  const uint8_t* p = nullptr;
+  int64_t rs = 0, cs = 0;
+};
+
+MaskArg mask_of(const OptTensor& mask, const Tensor& like, int64_t n, int64_t K) {
+  MaskArg m;
+  if (!has(mask)) return m;
+  TORCH_CHECK(mask->device() == like.device() && mask->scalar_type() == at::kBool &&
+                  mask->dim() == 2 && mask->size(0) == n && mask->size(1) == K,
+              "tdc.topk_gate: mask must be bool [N, K] on the scores' device");
+  m.p = static_cast<const uint8_t*>(mask->data_ptr());
+  m.rs = mask->stride(0);
+  m.cs = mask->stride(1);
+  return m;
+}
+
+std::vector<Tensor> topk_gate(const Tensor& scores, const OptTensor& mask, int64_t k, bool normalize,
+                              bool want_stat) {
+  check_rows(scores, "scores");
+  const int64_t n = scores.size(0), K = scores.size(1);
+  const int code = code_of(scores.scalar_type(), "scores");
+  TORCH_CHECK(k >= 1 && k <= 16 && k <= K && K <= MAX_SLOTS && n <= MAX_SLOTS,
+              "tdc.topk_gate: 1 to 16 of the clusters, got k = ", k, " of ", K);
+  const MaskArg m = mask_of(mask, scores, n, K);
+  const DevGuard guard(scores.device());
+  Tensor w = at::empty({n, k}, scores.options().dtype(at::kFloat));
+  Tensor labels = at::empty({n, k}, scores.options().dtype(at::kInt));
+  std::vector<Tensor> res = {w, labels};
+  Tensor stat;
+  if (want_stat) {
+    stat = at::empty({n, 2}, scores.options().dtype(at::kFloat));
+    res.push_back(stat);
+  }
+  check(tdc_topk_gate(code, scores.data_ptr(), scores.stride(0), m.p, m.rs, m.cs, n, (int)K, (int)k,
+                      normalize, w.data_ptr<float>(), labels.data_ptr<int32_t>(),
+                      stat.defined() ? stat.data_ptr<float>() : nullptr, cur_stream()),
+        "topk_gate");
+  return res;
+}
+
+// scores, mask, stat: given without `normalize` only.
+Tensor topk_gate_bwd(const OptTensor& scores, const OptTensor& mask, const Tensor& w,
+                     const Tensor& labels, const OptTensor& stat, const Tensor& dw, int64_t K,
+                     at::ScalarType dtype) {
+  TORCH_CHECK(w.is_cuda() && w.dim() == 2 && w.scalar_type() == at::kFloat && w.is_contiguous(),
+              "tdc.topk_gate_bwd: w fp32 [N, k]");
+  const int64_t n = w.size(0), k = w.size(1);
+  check_index(labels, w, n * k, "labels");
+  TORCH_CHECK(dw.device() == w.device() && dw.scalar_type() == at::kFloat && dw.is_contiguous() &&
+                  dw.numel() == n * k, "tdc.topk_gate_bwd: dw fp32 [N, k]");
+  const int code = code_of(dtype, "scores");
+  const bool normalize = !has(scores);
+  MaskArg m;
+  if (!normalize) {
+    check_rows(*scores, "scores");
+    TORCH_CHECK(scores->device() == w.device() && scores->scalar_type() == dtype &&
+                    scores->size(0) == n && scores->size(1) == K, "tdc.topk_gate_bwd: scores");
+    TORCH_CHECK(has(stat) && stat->device() == w.device() && stat->scalar_type() == at::kFloat &&
+                    stat->is_contiguous() && stat->numel() == 2 * n, "tdc.topk_gate_bwd: stat");
+    m = mask_of(mask, *scores, n, K);
+  }
+  const DevGuard guard(w.device());
+  Tensor ds = at::empty({n, K}, w.options().dtype(dtype));
+  check(tdc_topk_gate_bwd(code, normalize ? nullptr : scores->data_ptr(),
+                          normalize ? 0 : scores->stride(0), m.p, m.rs, m.cs, w.data_ptr<float>(),
+                          labels.data_ptr<int32_t>(), normalize ? nullptr : stat->data_ptr<float>(),
+                          dw.data_ptr<float>(), n, (int)K, (int)k, normalize, ds.data_ptr(),
+                          cur_stream()),
+        "topk_gate_bwd");
+  return ds;
+}
+
+// ------------------------------------------------------------------ groups
+std::vector<Tensor> group_plan(const Tensor& labels, int64_t K) {
+  TORCH_CHECK(labels.is_cuda() && labels.is_contiguous() &&
+                  (labels.scalar_type() == at::kInt || labels.scalar_type() == at::kLong),
+              "tdc.group_plan: labels must be contiguous int32 or int64 on the GPU");
+  const int64_t m = labels.numel();
+  TORCH_CHECK(K >= 1 && K < (1 << 22), "tdc.group_plan: 1 to 2^22 - 1 clusters, got ", K);
+  TORCH_CHECK(m <= MAX_SLOTS, "tdc.group_plan: too many labels: ", m);
+  const DevGuard guard(labels.device());
+  const auto opt = labels.options().dtype(at::kInt);
+  Tensor offsets = at::empty({K + 1}, opt);
+  Tensor order = at::empty({m}, opt);
+  Tensor pos = at::empty(labels.sizes(), opt);
+  const int64_t words = tdc_group_plan_work(m, (int)K);
+  Tensor work;
+  if (words) work = at::empty({words}, opt);
+  check(tdc_group_plan(labels.scalar_type() == at::kLong, labels.data_ptr(), m, (int)K,
+                       words ? work.data_ptr<int32_t>() : nullptr, order.data_ptr<int32_t>(),
+                       pos.data_ptr<int32_t>(), offsets.data_ptr<int32_t>(), cur_stream()),
+        "group_plan");
+  return {offsets, order, pos};
+}
+
+// pos int32 [N, k] or [N]: the slots of each row.
+int64_t slots_of(const Tensor& offsets, const Tensor& pos, const Tensor& like) {
+  TORCH_CHECK((pos.dim() == 1 || pos.dim() == 2) && offsets.dim() == 1 && offsets.numel() >= 2,
+              "tdc: pos [N] or [N, k], offsets [K + 1]");
+  check_index(offsets, like, offsets.numel(), "offsets");
+  check_index(pos, like, pos.numel(), "pos");
+  TORCH_CHECK(pos.numel() <= MAX_SLOTS, "tdc: too many slots");
+  return pos.dim() == 1 ? 1 : pos.size(1);
+}
+
+Tensor group_rows(const Tensor& x, const Tensor& offsets, const Tensor& pos) {
+  check_rows(x, "x");
+  const int64_t n = x.size(0), d = x.size(1), k = slots_of(offsets, pos, x);
+  const int code = code_of(x.scalar_type(), "x");
+  TORCH_CHECK(pos.size(0) == n && d >= 1 && d <= MAX_SLOTS, "tdc.group_rows: rows do not fit the plan");
+  const DevGuard guard(x.device());
+  Tensor out = at::empty({n * k, d}, x.options());
+  check(tdc_group_rows(code, x.data_ptr(), x.stride(0), n, (int)k, (int)d,
+                       offsets.data_ptr<int32_t>(), (int)offsets.numel() - 1,
+                       pos.data_ptr<int32_t>(), out.data_ptr(), cur_stream()),
+        "group_rows");
+  return out;
+}
+
+Tensor combine_rows(const Tensor& y, const Tensor& offsets, const Tensor& pos, const OptTensor& w) {
+  check_rows(y, "y");
+  const int64_t n = pos.size(0), d = y.size(1), k = slots_of(offsets, pos, y);
+  const int code = code_of(y.scalar_type(), "y");
+  TORCH_CHECK(y.size(0) == n * k && d >= 1 && d <= MAX_SLOTS, "tdc.combine_rows: rows do not fit the plan");
+  bool w32;
+  const void* wp = weights_of(w, y, n * k, w32);
+  const DevGuard guard(y.device());
+  Tensor out = at::empty({n, d}, y.options());
+  check(tdc_combine_rows(code, y.data_ptr(), y.stride(0), n, (int)k, (int)d,
+                         offsets.data_ptr<int32_t>(), (int)offsets.numel() - 1,
+                         pos.data_ptr<int32_t>(), wp, w32, out.data_ptr(), cur_stream()),
+        "combine_rows");
+  return out;
+}
+
+// y: given where the weights' gradient is wanted.
+std::vector<Tensor> combine_rows_bwd(const Tensor& dout, const OptTensor& y, const Tensor& offsets,
+                                     const Tensor& pos, const OptTensor& w, bool want_dy) {
+  check_rows(dout, "dout");
+  const int64_t n = dout.size(0), d = dout.size(1), k = slots_of(offsets, pos, dout);
+  const int code = code_of(dout.scalar_type(), "dout");
+  TORCH_CHECK(pos.size(0) == n && d >= 1 && d <= MAX_SLOTS,
+              "tdc.combine_rows_bwd: rows do not fit the plan");
+  bool w32;
+  const void* wp = weights_of(w, dout, n * k, w32);
+  const bool want_dw = has(y);
+  if (want_dw) {
+    check_rows(*y, "y");
+    TORCH_CHECK(wp != nullptr || n * k == 0, "tdc.combine_rows_bwd: dw needs the weights");
+    TORCH_CHECK(has(w) && y->device() == dout.device() && y->scalar_type() == dout.scalar_type() &&
+                    y->size(0) == n * k && y->size(1) == d, "tdc.combine_rows_bwd: y");
+  }
+  const DevGuard guard(dout.device());
+  Tensor dy, dw;
+  std::vector<Tensor> res;
+  if (want_dy) {
+    dy = at::empty({n * k, d}, dout.options());
+    res.push_back(dy);
+  }
+  if (want_dw) {
+    dw = at::empty(w->sizes(), w->options());
+    res.push_back(dw);
+  }
+  check(tdc_combine_rows_bwd(code, dout.data_ptr(), dout.stride(0),
+                             want_dw ? y->data_ptr() : nullptr, want_dw ? y->stride(0) : 0, n,
+                             (int)k, (int)d, offsets.data_ptr<int32_t>(), (int)offsets.numel() - 1,
+                             pos.data_ptr<int32_t>(), wp, w32, want_dy ? dy.data_ptr() : nullptr,
+                             want_dw ? dw.data_ptr() : nullptr, cur_stream()),
+        "combine_rows_bwd");
+  return res;
+}
+
+}  // namespace
+
+TORCH_LIBRARY_FRAGMENT(tdc, m) {
+  m.def("rms_norm(Tensor x, Tensor? w, Tensor? r, float eps, bool want_rstd, int fp8_width) -> Tensor[]");
+  m.def("rms_norm_bwd(Tensor h, Tensor? w, Tensor rstd, Tensor dy, Tensor? dh, bool want_dw) -> Tensor[]");
+  m.def("dequant_fp8(Tensor q, Tensor s, int d, ScalarType dtype) -> Tensor");
+  m.def("topk_gate(Tensor scores, Tensor? mask, int k, bool normalize, bool want_stat) -> Tensor[]");
+  m.def("topk_gate_bwd(Tensor? scores, Tensor? mask, Tensor w, Tensor labels, Tensor? stat, Tensor dw, int K, ScalarType dtype) -> Tensor");
+  m.def("group_plan(Tensor labels, int K) -> Tensor[]");
+  m.def("group_rows(Tensor x, Tensor offsets, Tensor pos) -> Tensor");
+  m.def("combine_rows(Tensor y, Tensor offsets, Tensor pos, Tensor? w) -> Tensor");
+  m.def("combine_rows_bwd(Tensor dout, Tensor? y, Tensor offsets, Tensor pos, Tensor? w, bool want_dy) -> Tensor[]");
+}
+
+TORCH_LIBRARY_IMPL(tdc, CUDA, m) {
+  m.impl("rms_norm", &rms_norm);
+  m.impl("rms_norm_bwd", &rms_norm_bwd);
+  m.impl("dequant_fp8", &dequant_fp8);
+  m.impl("topk_gate", &topk_gate);
+  m.impl("topk_gate_bwd", &topk_gate_bwd);
+  m.impl("group_plan", &group_plan);
+  m.impl("group_rows", &group_rows);
+  m.impl("combine_rows", &combine_rows);
+  m.impl("combine_rows_bwd", &combine_rows_bwd);
+}

@@ -6,7 +6,7 @@
 #include <stdint.h>
 
 // dtype codes shared with the bindings
-enum TdcDtype { TDC_F32 = 0, TDC_F64 = 1, TDC_BF16 = 2, TDC_FP8 = 3, TDC_I64 = 4 };
+enum TdcDtype { TDC_F32 = 0, TDC_F64 = 1, TDC_BF16 = 2, TDC_FP8 = 3, TDC_I64 = 4, TDC_F16 = 5 };
 // TDC_I64 as an accumulation dtype = fixed point (the deterministic update): partial sums
 // of round-toward-zero(x * fixed_scale) in int64 (fixed_scale a power of two chosen by the
 // caller so that every |sum| < 2^62); integer sums do not depend on the order of the
@@ -234,6 +234,52 @@ int tdc_assign_bigd_supported(int dtype, int DP);
 // neg2 != 0: centroid operand (-2c; norm of +c).  Rows >= valid are padding.
 int tdc_quant_fp8(int src_dtype, const void* X, int64_t rows, int64_t valid, int d, int64_t ldx,
                   int DP, int neg2, void* Q, void* S, float* norm, hipStream_t stream);
+
+// ---------------------------------------------------------------- row operators
+// dtype of rows: TDC_F32 / TDC_F16 / TDC_BF16; strides (ld*) in elements; w32: the weights are
+// fp32 (else of the rows' type).
+// RMS norm (rows_norm.hip): h = x + r in the rows' type (r nullable: h = x, not written), y or,
+// with q, e4m3 [n, dp] + E8M0 s [n, dp / 32] = h rstd w; rstd (nullable) fp32 [n]; d <= 16384.
+int tdc_rms_norm(int dtype, const void* x, int64_t ldx, const void* r, int64_t ldr, const void* w,
+                 int w32, int64_t n, int d, float eps, void* y, void* q, void* s, int dp, void* h,
+                 float* rstd, hipStream_t stream);
+// dx [n, d] (+ dh, nullable) and, with dw, dw [d] through part fp32 [parts, d] scratch.
+int tdc_rms_norm_bwd_parts(int64_t n, int cus);
+int tdc_rms_norm_bwd(int dtype, const void* h, int64_t ldh, const float* rstd, const void* w,
+                     int w32, const void* dy, int64_t lddy, const void* dh, int64_t lddh,
+                     int64_t n, int d, void* dx, float* part, int parts, void* dw,
+                     hipStream_t stream);
+// out [n, d] = q 2^(s - 127)
+int tdc_dequant_fp8(int dtype, const void* q, const void* s, int64_t n, int d, int dp, void* out,
+                    hipStream_t stream);
+// Top-k gate (rows_gate.hip), k <= 16: w fp32 [n, k], labels int32 [n, k] (-1: none), stat
+// (nullable) fp32 [n, 2] = largest score, 1 / sum of exponentials; mask (nullable) bytes,
+// nonzero = allowed, with row and column strides.
+int tdc_topk_gate(int dtype, const void* scores, int64_t ld, const uint8_t* mask, int64_t mask_rs,
+                  int64_t mask_cs, int64_t n, int K, int k, int normalize, float* w, int* labels,
+                  float* stat, hipStream_t stream);
+// ds [n, K] in the scores' type; scores, mask and stat are read without normalize only.
+int tdc_topk_gate_bwd(int dtype, const void* scores, int64_t ld, const uint8_t* mask,
+                      int64_t mask_rs, int64_t mask_cs, const float* w, const int* labels,
+                      const float* stat, const float* dw, int64_t n, int K, int k, int normalize,
+                      void* ds, hipStream_t stream);
+// Plan of rows by cluster (rows_group.hip): stable sort of m slots by label (int32, or int64
+// with wide_labels), K < 2^22; order / pos int32 [m], offsets int32 [K + 1]; work: int32
+// [tdc_group_plan_work(m, K)].
+int64_t tdc_group_plan_work(int64_t m, int K);
+int tdc_group_plan(int wide_labels, const void* labels, int64_t m, int K, int* work, int* order,
+                   int* pos, int* offsets, hipStream_t stream);
+// out [n k, d]: row n at the places of its k slots, zeros from offsets[K] on.
+int tdc_group_rows(int dtype, const void* x, int64_t ldx, int64_t n, int k, int d,
+                   const int* offsets, int K, const int* pos, void* out, hipStream_t stream);
+// out [n, d] = sum_j w[n, j] y[pos[n, j]] (w nullable: 1)
+int tdc_combine_rows(int dtype, const void* y, int64_t ldy, int64_t n, int k, int d,
+                     const int* offsets, int K, const int* pos, const void* w, int w32, void* out,
+                     hipStream_t stream);
+// dy [n k, d] and dw [n, k] (each nullable; y is read for dw only)
+int tdc_combine_rows_bwd(int dtype, const void* dout, int64_t lddo, const void* y, int64_t ldy,
+                         int64_t n, int k, int d, const int* offsets, int K, const int* pos,
+                         const void* w, int w32, void* dy, void* dw, hipStream_t stream);
 
 // N7 k-means++ step (kmeanspp.hip).  cand [T, D] (d_dtype, T <= 16), closest [N] (d_dtype).
 // mode 0: pots[t] += sum_i min(closest_i, ||x_i - cand_t||^2) for every candidate;

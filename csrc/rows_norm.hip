@@ -1,0 +1,355 @@
+// Root-mean-square norm of rows with the residual's addition, to the rows' own type or to
+// the block-scaled fp8 operand of the wide assignment, its gradient, and the way back from
+// fp8.
+//
+//   h = x + r                   rounded to the rows' type: the caller keeps it, and the
+//                               norm and its gradient are those of the kept row
+//   rstd = 1 / sqrt(mean h^2 + eps);  y = h * rstd * w
+//   gradient: g = dy * w, t = h * rstd, c = mean(g t):  dx = dr = rstd (g - t c) + dh,
+//             dw = sum over rows of dy t
+//   fp8: per 32 columns e = floor(log2 max|y|) - 7, q = e4m3(y 2^-e) (the layout of
+//        quant_fp8_kernel), columns past the row's end are zero
+//
+// All sums are fp32; y, h and dx are rounded once.  Bound by memory: the row lives in
+// registers between its one read and its one write.  A row is spread over G threads with
+// NV vectors of 16 bytes each; several rows share a wave when they are short, a block
+// works on one row when it is long.
+#include "rows_common.h"
+
+namespace tdc {
+namespace rows {
+
+constexpr int BLOCK = 256;
+
+template <int G> constexpr int block_of() { return G > BLOCK ? G : BLOCK; }
+
+template <typename T>
+__device__ __forceinline__ void load_weight(const void* __restrict__ w, bool w32, int c, int d,
+                                            float (&v)[Vec<T>::N]) {
+  if (w == nullptr) {
+#pragma unroll
+    for (int i = 0; i < Vec<T>::N; ++i) v[i] = 1.f;
+  } else if (w32) {
+    load_f32<Vec<T>::N>((const float*)w, c, d, v);
+  } else {
+    load_vec<T>((const T*)w, c, d, v);
+  }
+}
+
+// N values of one lane to e4m3 with the exponent of their block of 32 columns (32 / N
+// neighbouring lanes).  The block's largest value lies in [2^7, 2^8) after the scaling:
+// no saturation.
+template <int N>
+__device__ __forceinline__ void store_fp8(uint8_t* __restrict__ q, uint8_t* __restrict__ s, int c,
+                                          const float (&y)[N]) {
+  float am = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) am = fmaxf(am, fabsf(y[i]));
+#pragma unroll
+  for (int o = 1; o < 32 / N; o <<= 1) am = fmaxf(am, __shfl_xor(am, o, 64));
+  int e = am > 0.f ? ilogbf(am) - 7 : -127;
+  e = e < -127 ? -127 : (e > 126 ? 126 : e);
+  const float inv = ldexpf(1.f, -e);
+  int p[N / 4];
+#pragma unroll
+  for (int i = 0; i < N / 4; ++i) {
+    p[i] = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * i] * inv, y[4 * i + 1] * inv, 0, false);
+    p[i] = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * i + 2] * inv, y[4 * i + 3] * inv, p[i], true);
+  }
+  if constexpr (N == 8)
+    *reinterpret_cast<int2*>(q + c) = make_int2(p[0], p[1]);
+  else
+    *reinterpret_cast<int*>(q + c) = p[0];
+  if (c % 32 == 0) s[c / 32] = (uint8_t)(e + 127);
+}
+
+template <typename T, int G, int NV, bool FP8>
+__global__ __launch_bounds__(block_of<G>()) void norm_kernel(
+    const T* __restrict__ x, int64_t ldx, const T* __restrict__ r, int64_t ldr,
+    const void* __restrict__ w, bool w32, int64_t n, int d, float eps, T* __restrict__ y,
+    uint8_t* __restrict__ q, uint8_t* __restrict__ s, int dp, T* __restrict__ h,
+    float* __restrict__ rstd) {
+  constexpr int N = Vec<T>::N;
+  __shared__ float part[2][16];
+  int turn = 0;
+  const int lane = threadIdx.x % G;
+  const int64_t row = (int64_t)blockIdx.x * (block_of<G>() / G) + threadIdx.x / G;
+  if (row >= n) return;  // whole groups; G > 64: the block is one row of the grid
+  float v[NV][N];
+  float sq = 0.f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * G + lane) * N;
+    load_vec<T>(x + row * ldx, c, d, v[i]);
+  }
+  if (r) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * G + lane) * N;
+      float t[N];
+      load_vec<T>(r + row * ldr, c, d, t);
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[i][j] = up(down<T>(v[i][j] + t[j]));
+      store_vec<T>(h + row * d, c, d, v[i]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int j = 0; j < N; ++j) sq = fmaf(v[i][j], v[i][j], sq);
+  sq = group_sum<G>(sq, part, turn);
+  const float rs = 1.f / sqrtf(sq / (float)d + eps);
+  if (rstd && lane == 0) rstd[row] = rs;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * G + lane) * N;
+    float t[N];
+    load_weight<T>(w, w32, c, d, t);
+#pragma unroll
+    for (int j = 0; j < N; ++j) t[j] = v[i][j] * rs * t[j];
+    if constexpr (FP8) {
+      // the exponent's lanes all take part; a block of 32 is stored or not as a whole
+#pragma unroll
+      for (int j = 0; j < N; ++j) t[j] = c + j < d ? t[j] : 0.f;
+      if (c < dp) store_fp8<N>(q + row * dp, s + row * (dp / 32), c, t);
+    } else {
+      store_vec<T>(y + row * d, c, d, t);
+    }
+  }
+}
+
+// The gradient.  A block goes over rows with a stride of the grid and keeps its share of dw
+// in registers; the shares of its row groups are added in LDS order and leave as one row of
+// `part`, which dw_kernel sums: no atomics, the same order in every run.
+template <typename T, int G, int NV>
+__global__ __launch_bounds__(block_of<G>()) void norm_bwd_kernel(
+    const T* __restrict__ h, int64_t ldh, const float* __restrict__ rstd, const void* __restrict__ w,
+    bool w32, const T* __restrict__ dy, int64_t lddy, const T* __restrict__ dh, int64_t lddh,
+    int64_t n, int d, T* __restrict__ dx, float* __restrict__ part) {
+  constexpr int N = Vec<T>::N;
+  constexpr int GROUPS = block_of<G>() / G;
+  __shared__ float sums[2][16];
+  __shared__ float fold[GROUPS > 1 ? GROUPS : 1][GROUPS > 1 ? NV * G * N : 1];
+  int turn = 0;
+  const int lane = threadIdx.x % G, group = threadIdx.x / G;
+  float dw[NV][N];
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int j = 0; j < N; ++j) dw[i][j] = 0.f;
+  for (int64_t row = (int64_t)blockIdx.x * GROUPS + group; row < n;
+       row += (int64_t)gridDim.x * GROUPS) {
+    const float rs = rstd[row];
+    float t[NV][N], g[NV][N];
+    float dot = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * G + lane) * N;
+      load_vec<T>(h + row * ldh, c, d, t[i]);
+      load_vec<T>(dy + row * lddy, c, d, g[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      float wv[N];
+      load_weight<T>(w, w32, (i * G + lane) * N, d, wv);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        t[i][j] *= rs;
+        dw[i][j] = fmaf(g[i][j], t[i][j], dw[i][j]);
+        g[i][j] *= wv[j];
+        dot = fmaf(g[i][j], t[i][j], dot);
+      }
+    }
+    const float c1 = group_sum<G>(dot, sums, turn) / (float)d;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * G + lane) * N;
+      float o[N];
+#pragma unroll
+      for (int j = 0; j < N; ++j) o[j] = rs * (g[i][j] - t[i][j] * c1);
+      if (dh) {
+        float e[N];
+        load_vec<T>(dh + row * lddh, c, d, e);
+#pragma unroll
+        for (int j = 0; j < N; ++j) o[j] += e[j];
+      }
+      store_vec<T>(dx + row * d, c, d, o);
+    }
+  }
+  if (!part) return;
+  float* out = part + (int64_t)blockIdx.x * d;
+  if constexpr (GROUPS > 1) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < N; ++j) fold[group][(i * G + lane) * N + j] = dw[i][j];
+    __syncthreads();
+    for (int c = threadIdx.x; c < d; c += block_of<G>()) {
+      float a = 0.f;
+      for (int k = 0; k < GROUPS; ++k) a += fold[k][c];
+      out[c] = a;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const int c = (i * G + lane) * N + j;
+        if (c < d) out[c] = dw[i][j];
+      }
+  }
+}
+
+// dw[c] = sum of part[0..rows)[c]: a block takes 64 columns, its 16 waves every 16th row.
+template <typename W>
+__global__ __launch_bounds__(1024) void dw_kernel(const float* __restrict__ part, int rows, int d,
+                                                  W* __restrict__ dw) {
+  __shared__ float s[16][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int c = blockIdx.x * 64 + lane;
+  float a = 0.f;
+  if (c < d)
+    for (int k = wave; k < rows; k += 16) a += part[(int64_t)k * d + c];
+  s[wave][lane] = a;
+  __syncthreads();
+  if (wave == 0 && c < d) {
+    a = 0.f;
+    for (int k = 0; k < 16; ++k) a += s[k][lane];
+    dw[c] = down<W>(a);
+  }
+}
+
+// q 2^e of 16 columns per thread.
+template <typename T>
+__global__ __launch_bounds__(BLOCK) void dequant_kernel(const uint8_t* __restrict__ q,
+                                                        const uint8_t* __restrict__ s, int64_t n,
+                                                        int d, int dp, T* __restrict__ out) {
+  constexpr int N = Vec<T>::N;
+  const int per = (d + 15) / 16;
+  const int64_t i = (int64_t)blockIdx.x * BLOCK + threadIdx.x;
+  const int64_t row = i / per;
+  const int c = (int)(i % per) * 16;
+  if (row >= n) return;
+  const uint4 raw = *reinterpret_cast<const uint4*>(q + row * dp + c);
+  const int e = (int)s[row * (dp / 32) + c / 32] - 127;
+  const unsigned p[4] = {raw.x, raw.y, raw.z, raw.w};
+  float v[16];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    v[4 * k] = ldexpf(__builtin_amdgcn_cvt_f32_fp8((int)p[k], 0), e);
+    v[4 * k + 1] = ldexpf(__builtin_amdgcn_cvt_f32_fp8((int)p[k], 1), e);
+    v[4 * k + 2] = ldexpf(__builtin_amdgcn_cvt_f32_fp8((int)p[k], 2), e);
+    v[4 * k + 3] = ldexpf(__builtin_amdgcn_cvt_f32_fp8((int)p[k], 3), e);
+  }
+#pragma unroll
+  for (int k = 0; k < 16 / N; ++k) {
+    float t[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) t[j] = v[k * N + j];
+    if (c + k * N < d) store_vec<T>(out + row * d, c + k * N, d, t);
+  }
+}
+
+// Calls f(G, NV) for a row of `vecs` vectors of 16 bytes: the fewest threads that hold it
+// in at most 4 vectors each, a wave from 17 vectors on, so that the row's sum needs no
+// barrier up to 256 vectors (4 KiB).
+template <typename F> int with_shape(int vecs, F&& f) {
+#define TDC_SHAPE(G, NV) f(std::integral_constant<int, G>(), std::integral_constant<int, NV>())
+  if (vecs <= 16) return TDC_SHAPE(16, 1);
+  if (vecs <= 64) return TDC_SHAPE(64, 1);
+  if (vecs <= 128) return TDC_SHAPE(64, 2);
+  if (vecs <= 256) return TDC_SHAPE(64, 4);
+  if (vecs <= 512) return TDC_SHAPE(256, 2);
+  if (vecs <= 1024) return TDC_SHAPE(256, 4);
+  if (vecs <= 2048) return TDC_SHAPE(1024, 2);
+  if (vecs <= 4096) return TDC_SHAPE(1024, 4);
+#undef TDC_SHAPE
+  return (int)hipErrorInvalidValue;
+}
+
+}  // namespace rows
+}  // namespace tdc
+
+using namespace tdc::rows;
+
+int tdc_rms_norm(int dtype, const void* x, int64_t ldx, const void* r, int64_t ldr, const void* w,
+                 int w32, int64_t n, int d, float eps, void* y, void* q, void* s, int dp, void* h,
+                 float* rstd, hipStream_t stream) {
+  if (n == 0) return 0;
+  return with_type(dtype, [&](auto t) {
+    using T = decltype(t);
+    const int width = q ? dp : d;
+    return with_shape((width + Vec<T>::N - 1) / Vec<T>::N, [&](auto g, auto nv) {
+      constexpr int G = decltype(g)::value, NV = decltype(nv)::value;
+      constexpr int B = block_of<G>();
+      const int64_t blocks = (n + B / G - 1) / (B / G);
+      if (blocks > 0x7fffffff) return (int)hipErrorInvalidValue;
+      auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(B), 0, stream, (const T*)x, ldx,
+                           (const T*)r, ldr, w, w32 != 0, n, d, eps, (T*)y, (uint8_t*)q,
+                           (uint8_t*)s, dp, (T*)h, rstd);
+      };
+      if (q)
+        go(norm_kernel<T, G, NV, true>);
+      else
+        go(norm_kernel<T, G, NV, false>);
+      TDC_CHECK_LAUNCH();
+      return 0;
+    });
+  });
+}
+
+// Rows of `part` that tdc_rms_norm_bwd fills (0: none needed).
+int tdc_rms_norm_bwd_parts(int64_t n, int cus) {
+  const int64_t most = (int64_t)cus * 4;
+  return (int)(n < most ? n : most);
+}
+
+int tdc_rms_norm_bwd(int dtype, const void* h, int64_t ldh, const float* rstd, const void* w,
+                     int w32, const void* dy, int64_t lddy, const void* dh, int64_t lddh,
+                     int64_t n, int d, void* dx, float* part, int parts, void* dw,
+                     hipStream_t stream) {
+  if (parts < 1 && n > 0) return (int)hipErrorInvalidValue;
+  return with_type(dtype, [&](auto t) {
+    using T = decltype(t);
+    int used = 0;
+    if (n > 0) {
+      const int rc = with_shape((d + Vec<T>::N - 1) / Vec<T>::N, [&](auto g, auto nv) {
+        constexpr int G = decltype(g)::value, NV = decltype(nv)::value;
+        constexpr int B = block_of<G>();
+        const int64_t blocks = (n + B / G - 1) / (B / G);
+        used = (int)(blocks < parts ? blocks : parts);
+        hipLaunchKernelGGL((norm_bwd_kernel<T, G, NV>), dim3(used), dim3(B), 0, stream,
+                           (const T*)h, ldh, rstd, w, w32 != 0, (const T*)dy, lddy, (const T*)dh,
+                           lddh, n, d, (T*)dx, dw ? part : nullptr);
+        TDC_CHECK_LAUNCH();
+        return 0;
+      });
+      if (rc) return rc;
+    }
+    if (dw) {
+      const dim3 grid((unsigned)((d + 63) / 64));
+      if (w32)
+        hipLaunchKernelGGL(dw_kernel<float>, grid, dim3(1024), 0, stream, part, used, d, (float*)dw);
+      else
+        hipLaunchKernelGGL(dw_kernel<T>, grid, dim3(1024), 0, stream, part, used, d, (T*)dw);
+      TDC_CHECK_LAUNCH();
+    }
+    return 0;
+  });
+}
+
+int tdc_dequant_fp8(int dtype, const void* q, const void* s, int64_t n, int d, int dp, void* out,
+                    hipStream_t stream) {
+  if (n == 0) return 0;
+  if (dp % 32 != 0 || d > dp) return (int)hipErrorInvalidValue;
+  const int64_t blocks = (n * ((d + 15) / 16) + BLOCK - 1) / BLOCK;
+  if (blocks > 0x7fffffff) return (int)hipErrorInvalidValue;
+  return with_type(dtype, [&](auto t) {
+    using T = decltype(t);
+    hipLaunchKernelGGL(dequant_kernel<T>, dim3((unsigned)blocks), dim3(BLOCK), 0, stream,
+                       (const uint8_t*)q, (const uint8_t*)s, n, d, dp, (T*)out);
+    TDC_CHECK_LAUNCH();
+    return 0;
+  });
+}

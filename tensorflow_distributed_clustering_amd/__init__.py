@@ -9,10 +9,13 @@ from .config import ClusterConfig
 from .models.kmeans import KMeans, ClusterResult
 from .models.fcm import FuzzyCMeans
 from .models.minibatch import MiniBatchKMeans
+from .ops.rows import (Fp8Rows, RowGroups, combine_rows, group_plan, group_rows, rms_norm,
+                       rms_norm_fp8, topk_gate)
 from .parallel.dist import Comm, init_comm, local_comm, shard_bounds
 from .serving import ClusterPredictor
 
 __version__ = "0.1.0"
 
 __all__ = ["ClusterConfig", "KMeans", "FuzzyCMeans", "MiniBatchKMeans", "ClusterResult",
-           "ClusterPredictor", "Comm", "init_comm", "local_comm", "shard_bounds", "__version__"]
+           "ClusterPredictor", "Fp8Rows", "RowGroups", "combine_rows", "group_plan", "group_rows",
+           "rms_norm", "rms_norm_fp8", "topk_gate", "Comm", "init_comm", "local_comm", "shard_bounds", "__version__"]

@@ -797,6 +797,17 @@ class HipFp8Lloyd(_GroupedAssign, _LocalOpsBase):
                 diff = self.x[s:e, : self.d].float() - Cf.index_select(0, labels[s:e].long())
                 mind[s:e] = diff.pow_(2).sum(1).to(mind.dtype)
 
+    def assign_quantised(self, q, scales, labels):
+        """Labels of rows that are already the operand (``Fp8Rows`` of the fp8 norm, width
+        :attr:`dp`): no quantiser launch.  The row norms only enter distances.  Scratch is
+        the call's own: a captured graph may hold the buffers of :meth:`assign`."""
+        n = q.shape[0]
+        kg = kgroup_tiles(self._row_bytes, self.kp, n, self.kgroup_bytes)
+        norms = torch.empty(n, dtype=torch.float32, device=self.device)
+        keys = torch.full((n,), -1, dtype=torch.int64, device=self.device) if kg else None
+        self.ops.assign_bigd(q, scales, norms, self.cm2, self.cs, self.cnorm, kg, labels, None,
+                             keys)
+
     def step(self, C, labels, mind, sums, counts):
         self.assign(C, labels, mind)
         self.update(self.x, labels, sums, counts)

@@ -173,3 +173,78 @@ def kmeanspp(x: torch.Tensor, k: int, generator: torch.Generator,
         pot = float(pots[best])
         centers.append(xd[int(idx[best])])
     return torch.stack(centers).to(x.dtype)
+
+
+# ----------------------------------------------------------------- row operators
+# The formulas of ops/rows.py in fp32 (differentiable by autograd): the CPU path.
+
+def rms_norm(x, weight, residual, eps: float):
+    h = x if residual is None else (x.float() + residual.float()).to(x.dtype)
+    y = _normed(h, weight, eps).to(x.dtype)
+    return y if residual is None else (y, h)
+
+
+def _normed(h, weight, eps: float):
+    hf = h.float()
+    y = hf / torch.sqrt(hf.square().mean(1, keepdim=True) + eps)
+    return y if weight is None else y * weight.float()
+
+
+def rms_norm_fp8(x, weight, residual, eps: float, width: int):
+    """(q e4m3 [N, width], scales uint8 [N, width / 32][, h]): exponent floor(log2 max) - 7
+    per 32 columns, as the GPU quantiser."""
+    h = x if residual is None else (x.float() + residual.float()).to(x.dtype)
+    y = torch.nn.functional.pad(_normed(h, weight, eps), (0, width - x.shape[1]))
+    b = y.view(y.shape[0], width // 32, 32)
+    top = b.abs().nan_to_num(nan=0.0, posinf=math.inf).amax(2, keepdim=True)
+    e = torch.frexp(top)[1] - 8
+    e = torch.where(top > 0, e, -127)
+    e = torch.where(top.isinf(), 126, e).clamp(-127, 126)
+    q = torch.ldexp(b, -e).to(torch.float8_e4m3fn).view(y.shape)
+    out = (q, (e + 127).to(torch.uint8).squeeze(2))
+    return out if residual is None else (*out, h)
+
+
+def dequant_fp8(q, scales, d: int):
+    e = scales.int().repeat_interleave(32, 1) - 127
+    return torch.ldexp(q.float(), e)[:, :d]
+
+
+def topk_gate(scores, k: int, mask, normalize: bool):
+    v = scores.float()
+    if mask is not None:
+        v = torch.where(mask, v, -math.inf)
+    at = torch.sort(v.detach(), dim=1, descending=True, stable=True)[1][:, :k]
+    chosen = v.gather(1, at)
+    there = chosen != -math.inf
+    best = torch.where(there[:, :1], chosen[:, :1], 0.0).detach()
+    e = torch.exp(chosen - best)
+    total = (e if normalize else torch.exp(v - best)).sum(1, keepdim=True)
+    weights = e / torch.where(total == 0, 1.0, total)
+    # a row of NaN weights still has none where nothing was chosen
+    weights = torch.where(there, weights, 0.0)
+    return weights, torch.where(there, at, -1).to(torch.int32)
+
+
+def group_plan(labels, n_clusters: int):
+    flat = labels.reshape(-1).long()
+    key = torch.where((flat >= 0) & (flat < n_clusters), flat, n_clusters)
+    skey, order = torch.sort(key, stable=True)
+    pos = torch.empty_like(order)
+    pos[order] = torch.arange(order.numel(), device=order.device)
+    offsets = torch.searchsorted(skey, torch.arange(n_clusters + 1, device=order.device))
+    return offsets.int(), order.int(), pos.view(labels.shape).int()
+
+
+def group_rows(x, offsets, order, pos):
+    k = 1 if pos.dim() == 1 else pos.shape[1]
+    kept = torch.arange(order.numel(), device=x.device)[:, None] < offsets[-1]
+    return torch.where(kept, x.float()[order.long() // k], 0.0).to(x.dtype)
+
+
+def combine_rows(y, offsets, pos, weights):
+    p = pos.long().view(pos.shape[0], 1 if pos.dim() == 1 else pos.shape[1])
+    back = torch.where((p < offsets[-1])[..., None], y.float()[p], 0.0)
+    if weights is not None:
+        back = back * weights.float().view(p.shape)[..., None]
+    return back.sum(1).to(y.dtype)

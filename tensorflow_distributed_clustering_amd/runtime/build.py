@@ -26,6 +26,9 @@ CSRC = REPO / "csrc"
 BUILD = REPO / "build" / "obj"
 OUT = PKG_DIR / "_C.so"
 ARCH = os.environ.get("TDC_OFFLOAD_ARCH", "gfx950")
+# rows_*.hip: scalar fp32 arithmetic only.  The other sources keep packed fp32 (two of them
+# write it by hand).
+SCALAR_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 ROCM = Path(os.environ.get("ROCM_PATH", "/opt/rocm"))
 
 
@@ -71,7 +74,8 @@ def build(force: bool = False, verbose: bool = True, jobs: int = 0) -> Path:
         obj = BUILD / (src.stem + ".hip.o")
         objs.append(obj)
         if force or _needs(obj, [src] + headers):
-            tasks.append([hipcc, f"--offload-arch={ARCH}", *common, "-c", str(src), "-o", str(obj)])
+            extra = SCALAR_FP32 if src.stem.startswith("rows_") else []
+            tasks.append([hipcc, f"--offload-arch={ARCH}", *common, *extra, "-c", str(src), "-o", str(obj)])
     for src in cpp_srcs:
         obj = BUILD / (src.stem + ".cpp.o")
         objs.append(obj)

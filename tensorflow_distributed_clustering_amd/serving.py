@@ -21,7 +21,8 @@ from typing import Dict, Optional, Tuple
 import numpy as np
 import torch
 
-from .ops import make_lloyd_ops
+from .ops import HipFp8Lloyd, make_lloyd_ops
+from .ops.rows import Fp8Rows, group_plan, group_rows
 
 
 class ClusterPredictor:
@@ -73,7 +74,10 @@ class ClusterPredictor:
         """Labels (int32 [B]) of the rows of ``x`` [B, D]; with ``return_distance`` also
         their squared distance to the chosen centroid (kernel arithmetic).  ``copy=False``
         returns the per-batch-size output buffers themselves (no extra kernel; valid until
-        the next request of the same size)."""
+        the next request of the same size).  ``x`` may be the :class:`Fp8Rows` of
+        ``rms_norm_fp8`` where the predictor is fp8: they are assigned as they are."""
+        if isinstance(x, Fp8Rows):
+            return self._predict_fp8(x, return_distance)
         x = torch.as_tensor(x)
         if x.dim() != 2 or x.shape[1] != self.d:
             raise ValueError(f"expected [B, {self.d}] rows, got {tuple(x.shape)}")
@@ -98,6 +102,36 @@ class ClusterPredictor:
         if return_distance:
             return lab, md
         return lab
+
+    def _predict_fp8(self, x: Fp8Rows, return_distance: bool):
+        if self.dtype != "fp8":
+            raise ValueError(f"fp8 rows need a predictor with dtype='fp8', this one is {self.dtype}")
+        if x.d != self.d or x.device != self.device:
+            raise ValueError(f"expected [B, {self.d}] rows on {self.device}, got "
+                             f"{tuple(x.shape)} on {x.device}")
+        if not isinstance(self.local, HipFp8Lloyd):
+            return self.predict(x.dequantize(), return_distance)
+        if x.q.shape[1] != self.local.dp:
+            raise ValueError(f"fp8 rows of {x.q.shape[1]} columns, the operand has {self.local.dp}")
+        lab = torch.empty(x.shape[0], dtype=torch.int32, device=self.device)
+        if x.shape[0]:
+            self.local.assign_quantised(x.q, x.scales, lab)
+        if return_distance:
+            d2, step = torch.empty(x.shape[0], device=self.device), max(1, (1 << 26) // self.d)
+            for i in range(0, x.shape[0], step):
+                part = Fp8Rows(x.q[i:i + step], x.scales[i:i + step], x.d).dequantize()
+                part -= self.C.float().index_select(0, lab[i:i + step].long())
+                d2[i:i + step] = part.square_().sum(1)
+            return lab, d2
+        return lab
+
+    def partition(self, x):
+        """The rows of ``x`` [B, D] (fp32, fp16 or bf16) sorted by their cluster, and the
+        :class:`RowGroups` that say which rows those are: ``rows[groups.offsets[c] :
+        groups.offsets[c + 1]]`` are cluster c's, in their order in ``x``."""
+        x = torch.as_tensor(x).to(self.device)
+        groups = group_plan(self.predict(x), self.k)
+        return group_rows(x, groups), groups
 
     def score(self, x) -> float:
         """Negative inertia of ``x`` against the centroids (sklearn convention)."""

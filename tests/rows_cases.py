@@ -1,0 +1,110 @@
+"""Oracles of the row operators in 64 bits, and the tolerances that follow from their types.
+
+half(t) is the largest relative error of one rounding to t.  The kernels' fp32 sums of n
+terms are off by at most about n * half(fp32) of the sum of magnitudes, in practice far
+less; SUM covers widths to 16384 with tree sums (log2 n + a few roundings, taken as 32).
+"""
+import torch
+
+DTYPES = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def half(t):
+    return torch.finfo(t).eps / 2
+
+
+SUM = 32 * half(torch.float32)
+
+
+def close(got, want, dtype, scale=None, factor=1.0):
+    """got (of dtype) against want (fp64): one rounding to dtype and fp32 arithmetic of
+    `factor` sums, relative to `scale` (default: the value itself); the smallest normal of
+    fp16 bounds what its subnormals lose."""
+    want = want.double().to(got.device)
+    scale = want.abs() if scale is None else scale.double().to(got.device)
+    tol = half(dtype) * want.abs() * 1.01 + factor * SUM * scale + torch.finfo(dtype).tiny * half(dtype) * 2
+    bad = ~((got.double() - want).abs() <= tol)
+    assert not bool(bad.any()), (
+        f"{int(bad.sum())} of {bad.numel()} off, worst "
+        f"{float(((got.double() - want).abs() / tol).nan_to_num(nan=1e9).max()):.3g} of the tolerance")
+
+
+def sum_kept(x, residual):
+    """h: the sum in fp32, rounded to the rows' type (exact sum, one rounding, for 16 bits
+    unless the fp32 sum is itself rounded, in the kernel alike)."""
+    return x if residual is None else (x.float() + residual.float()).to(x.dtype)
+
+
+def norm(h, weight, eps):
+    h = h.double()
+    t = h / torch.sqrt((h * h).mean(1, keepdim=True) + eps)
+    return t, (t if weight is None else t * weight.double())
+
+
+def norm_grads(h, weight, eps, dy, dh):
+    """(dx, scale of dx's terms, dw, scale of dw's terms) from the formula."""
+    h64, dy = h.double(), dy.double()
+    rstd = 1 / torch.sqrt((h64 * h64).mean(1, keepdim=True) + eps)
+    t = h64 * rstd
+    g = dy if weight is None else dy * weight.double()
+    c, ca = (g * t).mean(1, keepdim=True), (g * t).abs().mean(1, keepdim=True)
+    dx, scale = rstd * (g - t * c), rstd * (g.abs() + t.abs() * ca)
+    if dh is not None:
+        dx, scale = dx + dh.double(), scale + dh.double().abs()
+    return dx, scale, (dy * t).sum(0), (dy * t).abs().sum(0)
+
+
+def fp8(y64, width):
+    """(values, exponents) of rows in 64 bits as e4m3 with one exponent per 32 columns, and
+    half the distance of e4m3 values around each (what a rounding may move)."""
+    # on the CPU, where powers of two come out exact
+    b = torch.nn.functional.pad(y64.cpu(), (0, width - y64.shape[1])).view(y64.shape[0], width // 32, 32)
+    top = b.abs().amax(2, keepdim=True)
+    e = torch.where(top > 0, torch.frexp(top)[1] - 8, -127).clamp(-127, 126)
+    v = torch.ldexp(b, -e)
+    x = torch.where(v == 0, -6, torch.frexp(v)[1] - 1).clamp(min=-6)
+    step = torch.ldexp(torch.ones_like(v), x - 3)
+    q = torch.round(v / step) * step
+    flat = (y64.shape[0], width)
+    return (torch.ldexp(q, e).view(flat).to(y64.device), e.squeeze(2).to(y64.device),
+            torch.ldexp(step, e).view(flat).to(y64.device))
+
+
+def gate(scores, k, mask, normalize, dw=None):
+    """(weights, labels[, ds]) with the choice made one by one, as Python compares."""
+    v = scores.double()
+    n, clusters = v.shape
+    ok = (v != -torch.inf) if mask is None else (mask.expand(v.shape) & (v != -torch.inf))
+    rank = torch.where(v.isnan(), torch.inf, v)
+    rank2 = v.isnan().double()                      # NaN orders above +inf
+    weights = torch.zeros(n, k, dtype=torch.float64)
+    labels = torch.full((n, k), -1, dtype=torch.int32)
+    ds = torch.zeros(n, clusters, dtype=torch.float64)
+    for r in range(n):
+        idx = [c for c in range(clusters) if bool(ok[r, c])]
+        pick = sorted(idx, key=lambda c: (-float(rank2[r, c]), -float(rank[r, c]), c))[:k]
+        if not pick:
+            continue
+        of = pick if normalize else idx
+        p = torch.zeros(clusters, dtype=torch.float64)
+        p[of] = torch.softmax(v[r, of], 0)
+        labels[r, :len(pick)] = torch.tensor(pick, dtype=torch.int32)
+        weights[r, :len(pick)] = p[pick]
+        if dw is not None:
+            up = torch.zeros(clusters, dtype=torch.float64)
+            up[pick] = dw[r, :len(pick)].double()
+            ds[r] = p * (up - (p * up).sum())
+    return (weights, labels) if dw is None else (weights, labels, ds)
+
+
+def plan(labels, clusters):
+    flat = labels.reshape(-1).tolist()
+    key = [v if 0 <= v < clusters else clusters for v in flat]
+    order = sorted(range(len(key)), key=lambda i: key[i])
+    pos = [0] * len(key)
+    for p, i in enumerate(order):
+        pos[i] = p
+    offsets = [sum(1 for v in key if v < c) for c in range(clusters + 1)] if len(key) * clusters < 1 << 22 else \
+        torch.searchsorted(torch.tensor(sorted(key)), torch.arange(clusters + 1)).tolist()
+    t = lambda v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
+    return t(offsets), t(order), t(pos).view(labels.shape)
