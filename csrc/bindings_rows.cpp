@@ -1,7 +1,12 @@
 // torch.ops.tdc.* of the row operators (rows_*.hip).  Unlike the iteration's ops, which write
 // into buffers of the engine, these return new tensors: a request is one call from Python,
-// and under graph capture the allocations belong to the graph's own pool.
+// and under graph capture the allocations belong to the graph's own pool.  The gradients are
+// C++ nodes: the autograd engine's worker thread runs them without the interpreter (measured
+// with rms_norm of 4 x 64 rows, forward and torch.autograd.grad: 59 us against 83 us with
+// nodes in Python).
 #include <torch/extension.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <ATen/hip/HIPContext.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
@@ -77,8 +82,8 @@ int num_cus(const Tensor& t) {
 }
 
 // ------------------------------------------------------------------ norm
-std::vector<Tensor> rms_norm(const Tensor& x, const OptTensor& w, const OptTensor& r, double eps,
-                             bool want_rstd, int64_t fp8_width) {
+std::vector<Tensor> norm_impl(const Tensor& x, const OptTensor& w, const OptTensor& r, double eps,
+                              bool want_rstd, int64_t fp8_width) {
   check_rows(x, "x");
   const int64_t n = x.size(0), d = x.size(1);
   const int code = code_of(x.scalar_type(), "x");
@@ -118,8 +123,8 @@ std::vector<Tensor> rms_norm(const Tensor& x, const OptTensor& w, const OptTenso
   return res;
 }
 
-std::vector<Tensor> rms_norm_bwd(const Tensor& h, const OptTensor& w, const Tensor& rstd,
-                                 const Tensor& dy, const OptTensor& dh, bool want_dw) {
+std::vector<Tensor> norm_bwd_impl(const Tensor& h, const OptTensor& w, const Tensor& rstd,
+                                  const Tensor& dy, const OptTensor& dh, bool want_dw) {
   check_rows(h, "h");
   check_like(dy, h, "dy");
   if (has(dh)) check_like(*dh, h, "dh");
@@ -184,7 +189,7 @@ MaskArg mask_of(const OptTensor& mask, const Tensor& like, int64_t n, int64_t K)
   return m;
 }
 
-std::vector<Tensor> topk_gate(const Tensor& scores, const OptTensor& mask, int64_t k, bool normalize,
+std::vector<Tensor> gate_impl(const Tensor& scores, const OptTensor& mask, int64_t k, bool normalize,
                               bool want_stat) {
   check_rows(scores, "scores");
   const int64_t n = scores.size(0), K = scores.size(1);
@@ -209,7 +214,7 @@ std::vector<Tensor> topk_gate(const Tensor& scores, const OptTensor& mask, int64
 }
 
 // scores, mask, stat: given without `normalize` only.
-Tensor topk_gate_bwd(const OptTensor& scores, const OptTensor& mask, const Tensor& w,
+Tensor gate_bwd_impl(const OptTensor& scores, const OptTensor& mask, const Tensor& w,
                      const Tensor& labels, const OptTensor& stat, const Tensor& dw, int64_t K,
                      at::ScalarType dtype) {
   TORCH_CHECK(w.is_cuda() && w.dim() == 2 && w.scalar_type() == at::kFloat && w.is_contiguous(),
@@ -273,7 +278,7 @@ int64_t slots_of(const Tensor& offsets, const Tensor& pos, const Tensor& like) {
   return pos.dim() == 1 ? 1 : pos.size(1);
 }
 
-Tensor group_rows(const Tensor& x, const Tensor& offsets, const Tensor& pos) {
+Tensor group_impl(const Tensor& x, const Tensor& offsets, const Tensor& pos) {
   check_rows(x, "x");
   const int64_t n = x.size(0), d = x.size(1), k = slots_of(offsets, pos, x);
   const int code = code_of(x.scalar_type(), "x");
@@ -287,7 +292,7 @@ Tensor group_rows(const Tensor& x, const Tensor& offsets, const Tensor& pos) {
   return out;
 }
 
-Tensor combine_rows(const Tensor& y, const Tensor& offsets, const Tensor& pos, const OptTensor& w) {
+Tensor combine_impl(const Tensor& y, const Tensor& offsets, const Tensor& pos, const OptTensor& w) {
   check_rows(y, "y");
   const int64_t n = pos.size(0), d = y.size(1), k = slots_of(offsets, pos, y);
   const int code = code_of(y.scalar_type(), "y");
@@ -304,7 +309,7 @@ Tensor combine_rows(const Tensor& y, const Tensor& offsets, const Tensor& pos, c
 }
 
 // y: given where the weights' gradient is wanted.
-std::vector<Tensor> combine_rows_bwd(const Tensor& dout, const OptTensor& y, const Tensor& offsets,
+std::vector<Tensor> combine_bwd_impl(const Tensor& dout, const OptTensor& y, const Tensor& offsets,
                                      const Tensor& pos, const OptTensor& w, bool want_dy) {
   check_rows(dout, "dout");
   const int64_t n = dout.size(0), d = dout.size(1), k = slots_of(offsets, pos, dout);
@@ -340,28 +345,204 @@ std::vector<Tensor> combine_rows_bwd(const Tensor& dout, const OptTensor& y, con
   return res;
 }
 
+// ------------------------------------------------------------------ autograd
+using torch::autograd::AutogradContext;
+using torch::autograd::Function;
+using torch::autograd::variable_list;
+
+bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
+bool wants_grad(const OptTensor& t) { return has(t) && t->requires_grad(); }
+
+// An incoming gradient in a layout that the kernels take (broadcast ones are laid out).
+Tensor laid_out(const Tensor& g) {
+  if (!g.defined() || g.size(1) <= 1 || g.stride(1) == 1) return g;
+  return g.contiguous();
+}
+
+// The gradients are not differentiable: asked for a graph, they give one that leads back to
+// what they were computed `from` and raises when it is used.
+variable_list once(variable_list grads, const variable_list& in, const variable_list& saved) {
+  if (!at::GradMode::is_enabled()) return grads;
+  variable_list have;
+  for (const Tensor& g : grads)
+    if (g.defined()) have.push_back(g);
+  for (const variable_list* from : {&in, &saved})
+    for (const Tensor& t : *from)
+      if (wants_grad(t)) have.push_back(t);
+  auto fn = std::make_shared<torch::autograd::DelayedError>(
+      "tdc: the gradients of the row operators are not differentiable", (int64_t)have.size());
+  have = (*fn)(std::move(have));
+  size_t i = 0;
+  for (Tensor& g : grads)
+    if (g.defined()) g = have[i++];
+  return grads;
+}
+
+OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; }
+
+struct RmsNorm : public Function<RmsNorm> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const OptTensor& w,
+                               const OptTensor& r, double eps) {
+    std::vector<Tensor> out = norm_impl(x, w, r, eps, true, 0);
+    Tensor rstd = out.back();
+    out.pop_back();
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({has(r) ? out[1] : x, has(w) ? *w : Tensor(), rstd});
+    ctx->saved_data["residual"] = has(r);
+    ctx->saved_data["dw"] = wants_grad(w);
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const bool residual = ctx->saved_data["residual"].toBool();
+    const bool want_dw = ctx->saved_data["dw"].toBool();
+    const Tensor dh = grads.size() > 1 ? laid_out(grads[1]) : Tensor();
+    variable_list res(4);
+    if (!grads[0].defined()) {  // only the sum was used
+      res[0] = dh;
+    } else {
+      const std::vector<Tensor> g =
+          norm_bwd_impl(saved[0], opt(saved[1]), saved[2], laid_out(grads[0]), opt(dh), want_dw);
+      res[0] = g[0];
+      if (want_dw) res[1] = g[1];
+    }
+    if (residual) res[2] = res[0];
+    return once(res, grads, saved);
+  }
+};
+
+struct TopkGate : public Function<TopkGate> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& scores, const OptTensor& mask,
+                               int64_t k, bool normalize) {
+    std::vector<Tensor> out = gate_impl(scores, mask, k, normalize, !normalize);
+    ctx->set_materialize_grads(false);
+    ctx->mark_non_differentiable({out[1]});
+    // the weights over the chosen say all about their gradient; those over every cluster
+    // need the scores again
+    if (normalize)
+      ctx->save_for_backward({out[0], out[1]});
+    else
+      ctx->save_for_backward({out[0], out[1], scores, out[2], has(mask) ? *mask : Tensor()});
+    ctx->saved_data["clusters"] = scores.size(1);
+    ctx->saved_data["dtype"] = (int64_t)scores.scalar_type();
+    return {out[0], out[1]};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list res(4);
+    if (!grads[0].defined()) return res;
+    const auto saved = ctx->get_saved_variables();
+    const bool normalize = saved.size() == 2;
+    res[0] = gate_bwd_impl(normalize ? std::nullopt : opt(saved[2]),
+                           normalize ? std::nullopt : opt(saved[4]), saved[0], saved[1],
+                           normalize ? std::nullopt : opt(saved[3]), grads[0].contiguous(),
+                           ctx->saved_data["clusters"].toInt(),
+                           (at::ScalarType)ctx->saved_data["dtype"].toInt());
+    return once(res, grads, saved);
+  }
+};
+
+struct GroupRows : public Function<GroupRows> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& offsets,
+                        const Tensor& pos) {
+    ctx->save_for_backward({offsets, pos});
+    return group_impl(x, offsets, pos);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    variable_list res(3);
+    res[0] = combine_impl(laid_out(grads[0]), saved[0], saved[1], std::nullopt);
+    return once(res, grads, saved);
+  }
+};
+
+struct CombineRows : public Function<CombineRows> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& y, const Tensor& offsets,
+                        const Tensor& pos, const OptTensor& w) {
+    ctx->save_for_backward({offsets, pos, has(w) ? *w : Tensor(), wants_grad(w) ? y : Tensor()});
+    ctx->saved_data["dy"] = wants_grad(y);
+    return combine_impl(y, offsets, pos, w);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const bool want_dy = ctx->saved_data["dy"].toBool();
+    const std::vector<Tensor> g = combine_bwd_impl(laid_out(grads[0]), opt(saved[3]), saved[0],
+                                                   saved[1], opt(saved[2]), want_dy);
+    variable_list res(4);
+    if (want_dy) res[0] = g[0];
+    if (saved[3].defined()) res[3] = g.back();
+    return once(res, grads, saved);
+  }
+};
+
+bool no_graph() { return !at::GradMode::is_enabled(); }
+
+std::vector<Tensor> rms_norm(const Tensor& x, const OptTensor& w, const OptTensor& r, double eps) {
+  return norm_impl(x, w, r, eps, false, 0);
+}
+std::vector<Tensor> rms_norm_ad(const Tensor& x, const OptTensor& w, const OptTensor& r, double eps) {
+  if (no_graph() || !(wants_grad(x) || wants_grad(w) || wants_grad(r))) return rms_norm(x, w, r, eps);
+  return RmsNorm::apply(x, w, r, eps);
+}
+
+std::vector<Tensor> rms_norm_fp8(const Tensor& x, const OptTensor& w, const OptTensor& r, double eps,
+                                 int64_t width) {
+  TORCH_CHECK(width > 0, "tdc.rms_norm_fp8: width");
+  return norm_impl(x, w, r, eps, false, width);
+}
+
+std::tuple<Tensor, Tensor> topk_gate(const Tensor& scores, const OptTensor& mask, int64_t k,
+                                     bool normalize) {
+  const std::vector<Tensor> out = gate_impl(scores, mask, k, normalize, false);
+  return {out[0], out[1]};
+}
+std::tuple<Tensor, Tensor> topk_gate_ad(const Tensor& scores, const OptTensor& mask, int64_t k,
+                                        bool normalize) {
+  if (no_graph() || !wants_grad(scores)) return topk_gate(scores, mask, k, normalize);
+  const variable_list out = TopkGate::apply(scores, mask, k, normalize);
+  return {out[0], out[1]};
+}
+
+Tensor group_rows(const Tensor& x, const Tensor& offsets, const Tensor& pos) {
+  return group_impl(x, offsets, pos);
+}
+Tensor group_rows_ad(const Tensor& x, const Tensor& offsets, const Tensor& pos) {
+  if (no_graph() || !wants_grad(x)) return group_impl(x, offsets, pos);
+  return GroupRows::apply(x, offsets, pos);
+}
+
+Tensor combine_rows(const Tensor& y, const Tensor& offsets, const Tensor& pos, const OptTensor& w) {
+  return combine_impl(y, offsets, pos, w);
+}
+Tensor combine_rows_ad(const Tensor& y, const Tensor& offsets, const Tensor& pos, const OptTensor& w) {
+  if (no_graph() || !(wants_grad(y) || wants_grad(w))) return combine_impl(y, offsets, pos, w);
+  return CombineRows::apply(y, offsets, pos, w);
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(tdc, m) {
-  m.def("rms_norm(Tensor x, Tensor? w, Tensor? r, float eps, bool want_rstd, int fp8_width) -> Tensor[]");
-  m.def("rms_norm_bwd(Tensor h, Tensor? w, Tensor rstd, Tensor dy, Tensor? dh, bool want_dw) -> Tensor[]");
+  m.def("rms_norm(Tensor x, Tensor? w, Tensor? r, float eps) -> Tensor[]");
+  m.def("rms_norm_fp8(Tensor x, Tensor? w, Tensor? r, float eps, int width) -> Tensor[]");
   m.def("dequant_fp8(Tensor q, Tensor s, int d, ScalarType dtype) -> Tensor");
-  m.def("topk_gate(Tensor scores, Tensor? mask, int k, bool normalize, bool want_stat) -> Tensor[]");
-  m.def("topk_gate_bwd(Tensor? scores, Tensor? mask, Tensor w, Tensor labels, Tensor? stat, Tensor dw, int K, ScalarType dtype) -> Tensor");
+  m.def("topk_gate(Tensor scores, Tensor? mask, int k, bool normalize) -> (Tensor, Tensor)");
   m.def("group_plan(Tensor labels, int K) -> Tensor[]");
   m.def("group_rows(Tensor x, Tensor offsets, Tensor pos) -> Tensor");
   m.def("combine_rows(Tensor y, Tensor offsets, Tensor pos, Tensor? w) -> Tensor");
-  m.def("combine_rows_bwd(Tensor dout, Tensor? y, Tensor offsets, Tensor pos, Tensor? w, bool want_dy) -> Tensor[]");
 }
 
 TORCH_LIBRARY_IMPL(tdc, CUDA, m) {
   m.impl("rms_norm", &rms_norm);
-  m.impl("rms_norm_bwd", &rms_norm_bwd);
+  m.impl("rms_norm_fp8", &rms_norm_fp8);
   m.impl("dequant_fp8", &dequant_fp8);
   m.impl("topk_gate", &topk_gate);
-  m.impl("topk_gate_bwd", &topk_gate_bwd);
   m.impl("group_plan", &group_plan);
   m.impl("group_rows", &group_rows);
   m.impl("combine_rows", &combine_rows);
-  m.impl("combine_rows_bwd", &combine_rows_bwd);
+}
+
+TORCH_LIBRARY_IMPL(tdc, AutogradCUDA, m) {
+  m.impl("rms_norm", &rms_norm_ad);
+  m.impl("topk_gate", &topk_gate_ad);
+  m.impl("group_rows", &group_rows_ad);
+  m.impl("combine_rows", &combine_rows_ad);
 }

@@ -22,7 +22,6 @@ import math
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _native
 from . import reference as ref
@@ -65,35 +64,7 @@ def _check_weight(w, x, shape, name: str):
         raise ValueError(f"{name} is on {w.device}, the rows on {x.device}")
 
 
-def _rows(g: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    """An incoming gradient in a layout the kernels take (broadcast ones are laid out)."""
-    if g is None or g.shape[1] == 1 or g.stride(1) == 1:
-        return g
-    return g.contiguous()
-
-
 # ----------------------------------------------------------------- norm
-class _RmsNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, residual, eps):
-        out = _ops().rms_norm(x, weight, residual, eps, True, 0)
-        ctx.set_materialize_grads(False)
-        h = x if residual is None else out[1]
-        ctx.save_for_backward(h, weight, out[-1])
-        ctx.with_residual = residual is not None
-        return out[0] if residual is None else (out[0], h)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy, dh=None):
-        h, weight, rstd = ctx.saved_tensors
-        want_dw = weight is not None and ctx.needs_input_grad[1]
-        if dy is None:  # only the sum was used
-            return dh, None, (dh if ctx.with_residual else None), None
-        grads = _ops().rms_norm_bwd(h, weight, rstd, _rows(dy), _rows(dh), want_dw)
-        return grads[0], (grads[1] if want_dw else None), (grads[0] if ctx.with_residual else None), None
-
-
 def _check_norm(x, weight, residual, eps):
     _check_rows(x, "x")
     if x.shape[1] > MAX_WIDTH:
@@ -120,10 +91,7 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
     _check_norm(x, weight, residual, eps)
     if x.device.type != "cuda":
         return ref.rms_norm(x, weight, residual, eps)
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
-                                    or (residual is not None and residual.requires_grad)):
-        return _RmsNorm.apply(x, weight, residual, eps)
-    out = _ops().rms_norm(x, weight, residual, eps, False, 0)
+    out = _ops().rms_norm(x, weight, residual, eps)
     return out[0] if residual is None else (out[0], out[1])
 
 
@@ -175,39 +143,12 @@ def rms_norm_fp8(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
     if x.device.type != "cuda":
         out = ref.rms_norm_fp8(x, weight, residual, eps, fp8_width(d))
     else:
-        out = _ops().rms_norm(x, weight, residual, eps, False, fp8_width(d))
+        out = _ops().rms_norm_fp8(x, weight, residual, eps, fp8_width(d))
     rows = Fp8Rows(out[0], out[1], d)
     return rows if residual is None else (rows, out[2])
 
 
 # ----------------------------------------------------------------- gate
-class _TopkGate(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, scores, mask, k, normalize):
-        out = _ops().topk_gate(scores, mask, k, normalize, not normalize)
-        w, labels = out[0], out[1]
-        ctx.mark_non_differentiable(labels)
-        ctx.set_materialize_grads(False)
-        # the weights over the chosen say all about their gradient; those over every
-        # cluster need the scores again
-        ctx.save_for_backward(w, labels, *(() if normalize else (scores, out[2], mask)))
-        ctx.shape = (scores.shape[1], scores.dtype, normalize)
-        return w, labels
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dw, _):
-        if dw is None:
-            return None, None, None, None
-        clusters, dtype, normalize = ctx.shape
-        if normalize:
-            (w, labels), scores, stat, mask = ctx.saved_tensors, None, None, None
-        else:
-            w, labels, scores, stat, mask = ctx.saved_tensors
-        ds = _ops().topk_gate_bwd(scores, mask, w, labels, stat, dw.contiguous(), clusters, dtype)
-        return ds, None, None, None
-
-
 def topk_gate(scores: torch.Tensor, k: int, mask: Optional[torch.Tensor] = None,
               normalize: bool = True) -> Tuple[torch.Tensor, torch.Tensor]:
     """The ``k`` clusters of the largest ``scores`` [N, K] of each row, 1 <= k <= min(16, K).
@@ -237,10 +178,7 @@ def topk_gate(scores: torch.Tensor, k: int, mask: Optional[torch.Tensor] = None,
     normalize = bool(normalize)
     if scores.device.type != "cuda":
         return ref.topk_gate(scores, k, mask, normalize)
-    if torch.is_grad_enabled() and scores.requires_grad:
-        return _TopkGate.apply(scores, mask, k, normalize)
-    w, labels = _ops().topk_gate(scores, mask, k, normalize, False)
-    return w, labels
+    return _ops().topk_gate(scores, mask, k, normalize)
 
 
 # ----------------------------------------------------------------- groups
@@ -297,19 +235,6 @@ def _check_groups(groups):
         raise TypeError(f"groups must be the RowGroups of group_plan, got {type(groups).__name__}")
 
 
-class _GroupRows(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, offsets, pos):
-        ctx.save_for_backward(offsets, pos)
-        return _ops().group_rows(x, offsets, pos)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dxg):
-        offsets, pos = ctx.saved_tensors
-        return _ops().combine_rows(_rows(dxg), offsets, pos, None), None, None
-
-
 def group_rows(x: torch.Tensor, groups: RowGroups) -> torch.Tensor:
     """The rows of ``x`` [N, D] sorted by cluster, [N * k, D]: a row once for each of its
     labels, zeros at the places from ``groups.offsets[-1]`` on.  The gradient sums a row's
@@ -321,25 +246,7 @@ def group_rows(x: torch.Tensor, groups: RowGroups) -> torch.Tensor:
                          f"x has {x.shape[0]} on {x.device}")
     if x.device.type != "cuda":
         return ref.group_rows(x, groups.offsets, groups.order, groups.pos)
-    if torch.is_grad_enabled() and x.requires_grad:
-        return _GroupRows.apply(x, groups.offsets, groups.pos)
     return _ops().group_rows(x, groups.offsets, groups.pos)
-
-
-class _CombineRows(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, y, offsets, pos, weights):
-        want_dw = weights is not None and ctx.needs_input_grad[3]
-        ctx.save_for_backward(offsets, pos, weights, y if want_dw else None)
-        return _ops().combine_rows(y, offsets, pos, weights)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dout):
-        offsets, pos, weights, y = ctx.saved_tensors
-        want_dy, want_dw = ctx.needs_input_grad[0], y is not None
-        grads = _ops().combine_rows_bwd(_rows(dout), y, offsets, pos, weights, want_dy)
-        return grads[0] if want_dy else None, None, None, (grads[-1] if want_dw else None)
 
 
 def combine_rows(y: torch.Tensor, groups: RowGroups, weights: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -356,6 +263,4 @@ def combine_rows(y: torch.Tensor, groups: RowGroups, weights: Optional[torch.Ten
         _check_weight(weights, y, groups.pos.shape, "weights")
     if y.device.type != "cuda":
         return ref.combine_rows(y, groups.offsets, groups.pos, weights)
-    if torch.is_grad_enabled() and (y.requires_grad or (weights is not None and weights.requires_grad)):
-        return _CombineRows.apply(y, groups.offsets, groups.pos, weights)
     return _ops().combine_rows(y, groups.offsets, groups.pos, weights)

@@ -123,6 +123,24 @@ def test_predictor_reads_fp8_rows(gpu):
         assert torch.equal(parts, x[:n][order]) and torch.equal(groups.order.long(), order)
 
 
+def test_gradients_are_not_differentiable(gpu):
+    x, w = normal(gpu, 1, 6, 40).requires_grad_(), normal(gpu, 2, 40).requires_grad_()
+    groups = tdc.group_plan(torch.zeros(6, dtype=torch.int32, device=gpu), 2)
+    v = torch.ones(6, device=gpu, requires_grad=True)
+    for out, leaves, again in ((tdc.rms_norm(x, w), (x, w), x), (tdc.topk_gate(x, 3)[0], (x,), x),
+                               (tdc.group_rows(x, groups), (x,), None),
+                               (tdc.combine_rows(x, groups, v), (x, v), v)):
+        up = torch.ones_like(out).requires_grad_()
+        plain = torch.autograd.grad(out, leaves, up.detach(), retain_graph=True)
+        grads = torch.autograd.grad(out, leaves, up, create_graph=True)
+        for g, e in zip(grads, plain):
+            assert torch.equal(g, e)
+            for of in (up, again):
+                if of is not None:
+                    with pytest.raises(RuntimeError, match="not differentiable"):
+                        torch.autograd.grad(g.square().sum(), of, retain_graph=True)
+
+
 # ----------------------------------------------------------------- gate
 @pytest.mark.parametrize("clusters,k", [(1, 1), (7, 7), (64, 2), (100, 16), (129, 3), (256, 8), (257, 6),
                                         (1000, 8), (1024, 16), (1025, 5), (4099, 16)])
