@@ -21,57 +21,104 @@ struct __attribute__((packed, aligned(2))) Raw16 { unsigned w[4]; };
 template <typename T> __device__ __forceinline__ float up(T v) { return (float)v; }
 template <typename T> __device__ __forceinline__ T down(float v) { return (T)v; }
 
-// Elements [c, c + Vec<T>::N) of a row of `width` as floats; those past its end are 0.
-// The row's last, partial vector is read element by element.
+template <typename T> __device__ __forceinline__ Raw16 load16(const T* p) {
+  return *reinterpret_cast<const Raw16*>(p);
+}
+template <typename T> __device__ __forceinline__ void store16(T* p, const Raw16& r) {
+  *reinterpret_cast<Raw16*>(p) = r;
+}
+// r, or zeros (word by word: a choice between two structs goes through scratch memory).
+__device__ __forceinline__ Raw16 if_kept(bool kept, const Raw16& r) {
+  Raw16 o;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o.w[i] = kept ? r.w[i] : 0u;
+  return o;
+}
 template <typename T>
-__device__ __forceinline__ void load_vec(const T* __restrict__ row, int c, int width,
-                                         float (&v)[Vec<T>::N]) {
-  constexpr int N = Vec<T>::N;
-  if (c + N <= width) {
-    const Raw16 raw = *reinterpret_cast<const Raw16*>(row + c);
-    T t[N];
-    __builtin_memcpy(t, &raw, 16);
+__device__ __forceinline__ void unpack(const Raw16& r, float (&v)[Vec<T>::N]) {
+  T t[Vec<T>::N];
+  __builtin_memcpy(t, &r, 16);
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = up(t[i]);
-  } else {
+  for (int i = 0; i < Vec<T>::N; ++i) v[i] = up(t[i]);
+}
+template <typename T> __device__ __forceinline__ Raw16 pack(const float (&v)[Vec<T>::N]) {
+  T t[Vec<T>::N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = c + i < width ? up(row[c + i]) : 0.f;
-  }
+  for (int i = 0; i < Vec<T>::N; ++i) t[i] = down<T>(v[i]);
+  Raw16 r;
+  __builtin_memcpy(&r, t, 16);
+  return r;
 }
 
-// The same for N fp32 values next to a vector of N elements of T (weights, partial sums).
-template <int N>
-__device__ __forceinline__ void load_f32(const float* __restrict__ row, int c, int width,
-                                         float (&v)[N]) {
-  static_assert(N % 4 == 0, "whole dwordx4");
-  if (c + N <= width) {
+// How a row of `width` splits into vectors of N elements: TAIL_NONE: without rest;
+// TAIL_SHIFT: its last vector is partial; TAIL_SHORT: it is shorter than one vector.
+// A load must not sit in a branch of its own lanes: the wait for it would sit there too,
+// and the loads of a thread would go out one after the other (measured on rows of 2 KiB
+// moved by place: 3.5 TB/s with a branch around each load, 5.9 without).
+enum Tail { TAIL_NONE = 0, TAIL_SHIFT = 1, TAIL_SHORT = 2 };
+
+// Elements [c, c + N) of a row; fetch() issues the load, value() gives the floats, 0 past
+// the row's end.  The last vector is read N elements before the end and shifted.
+template <typename T, int TAIL> struct RowVec {
+  static constexpr int N = Vec<T>::N;
+  static __device__ __forceinline__ Raw16 fetch(const T* __restrict__ row, int c, int width) {
+    if constexpr (TAIL == TAIL_SHORT) {
+      T t[N];
 #pragma unroll
-    for (int q = 0; q < N / 4; ++q) {
-      const Raw16 raw = *reinterpret_cast<const Raw16*>(row + c + 4 * q);
-      __builtin_memcpy(&v[4 * q], &raw, 16);
+      for (int i = 0; i < N; ++i) t[i] = c + i < width ? row[c + i] : T(0.f);
+      Raw16 r;
+      __builtin_memcpy(&r, t, 16);
+      return r;
+    } else {
+      return load16(row + min(c, width - N));
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = c + i < width ? row[c + i] : 0.f;
   }
-}
+  static __device__ __forceinline__ void value(Raw16 r, int c, int width, float (&v)[N]) {
+    if constexpr (TAIL == TAIL_SHIFT) {
+      const int by = (c - min(c, width - N)) * (int)sizeof(T);  // bytes to drop in front
+      unsigned long long lo, hi;
+      __builtin_memcpy(&lo, &r.w[0], 8);
+      __builtin_memcpy(&hi, &r.w[2], 8);
+      if (by >= 16) {
+        lo = hi = 0;
+      } else if (by >= 8) {
+        lo = hi >> (8 * (by - 8));
+        hi = 0;
+      } else if (by > 0) {
+        lo = (lo >> (8 * by)) | (hi << (64 - 8 * by));
+        hi >>= 8 * by;
+      }
+      __builtin_memcpy(&r.w[0], &lo, 8);
+      __builtin_memcpy(&r.w[2], &hi, 8);
+      unpack<T>(r, v);
+    } else {
+      unpack<T>(r, v);
+      if constexpr (TAIL == TAIL_NONE) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = c < width ? v[i] : 0.f;
+      }
+    }
+  }
+  static __device__ __forceinline__ void store(T* __restrict__ row, int c, int width,
+                                               const float (&v)[N]) {
+    const Raw16 r = pack<T>(v);
+    if (TAIL != TAIL_SHORT && c + N <= width) {
+      store16(row + c, r);
+    } else if (TAIL != TAIL_NONE && c < width) {
+      T t[N];
+      __builtin_memcpy(t, &r, 16);
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (c + i < width) row[c + i] = t[i];
+    }
+  }
+};
 
-template <typename T>
-__device__ __forceinline__ void store_vec(T* __restrict__ row, int c, int width,
-                                          const float (&v)[Vec<T>::N]) {
-  constexpr int N = Vec<T>::N;
-  T t[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) t[i] = down<T>(v[i]);
-  if (c + N <= width) {
-    Raw16 raw;
-    __builtin_memcpy(&raw, t, 16);
-    *reinterpret_cast<Raw16*>(row + c) = raw;
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (c + i < width) row[c + i] = t[i];
-  }
+// f(integral_constant<TAIL>) for a row of d elements in vectors of n.
+template <typename F> int with_tail(int d, int n, F&& f) {
+  if (d < n) return f(std::integral_constant<int, TAIL_SHORT>());
+  if (d % n) return f(std::integral_constant<int, TAIL_SHIFT>());
+  return f(std::integral_constant<int, TAIL_NONE>());
 }
 
 // Sum over G neighbouring lanes (a power of two up to 64), the same value in each.

@@ -40,7 +40,7 @@ struct Mask {
 
 // L lanes work on a row, each with R scores in registers.  Every round takes the largest
 // that is left, over the registers and then over the lanes.
-template <typename T, int L, int R>
+template <typename T, int L, int R, int TAIL>
 __global__ __launch_bounds__(GATE_BLOCK) void gate_kernel(const T* __restrict__ scores, int64_t ld,
                                                           Mask mask, int64_t n, int K, int k,
                                                           bool normalize, float* __restrict__ w,
@@ -52,11 +52,15 @@ __global__ __launch_bounds__(GATE_BLOCK) void gate_kernel(const T* __restrict__ 
   if (row >= n) return;
   unsigned key[R];
   unsigned best = 0;
+  Raw16 raw[R / V];
+#pragma unroll
+  for (int i = 0; i < R / V; ++i)
+    raw[i] = RowVec<T, TAIL>::fetch(scores + row * ld, (i * L + lane) * V, K);
 #pragma unroll
   for (int i = 0; i < R / V; ++i) {
     const int c = (i * L + lane) * V;
     float v[V];
-    load_vec<T>(scores + row * ld, c, K, v);
+    RowVec<T, TAIL>::value(raw[i], c, K, v);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       key[i * V + j] = order_of(v[j], c + j < K && mask.at(row, c + j));
@@ -190,7 +194,7 @@ __global__ __launch_bounds__(GATE_BLOCK) void gate_wide_kernel(
 
 // The gradient: L lanes per row write what every place gets and then, after those stores
 // have arrived, the chosen places.
-template <typename T, int L>
+template <typename T, int L, int TAIL>
 __global__ __launch_bounds__(GATE_BLOCK) void gate_bwd_kernel(
     const T* __restrict__ scores, int64_t ld, Mask mask, const float* __restrict__ w,
     const int* __restrict__ labels, const float* __restrict__ stat, const float* __restrict__ dw,
@@ -213,14 +217,14 @@ __global__ __launch_bounds__(GATE_BLOCK) void gate_bwd_kernel(
 #pragma unroll
     for (int j = 0; j < V; ++j) v[j] = 0.f;
     if (!normalize) {
-      load_vec<T>(scores + row * ld, c, K, v);
+      RowVec<T, TAIL>::value(RowVec<T, TAIL>::fetch(scores + row * ld, c, K), c, K, v);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         const bool in = c + j < K && mask.at(row, c + j) && v[j] != -INFINITY;
         v[j] = in ? -expf(v[j] - top) * scale : 0.f;
       }
     }
-    store_vec<T>(ds + row * K, c, K, v);
+    RowVec<T, TAIL>::store(ds + row * K, c, K, v);
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   if (at >= 0 && at < K) ds[row * K + at] = down<T>(wj * (dj - mean));
@@ -244,16 +248,19 @@ int tdc_topk_gate(int dtype, const void* scores, int64_t ld, const uint8_t* mask
       hipLaunchKernelGGL(kernel, dim3((unsigned)((n + rows - 1) / rows)), dim3(GATE_BLOCK), 0,
                          stream, (const T*)scores, ld, m, n, K, k, normalize != 0, w, labels, stat);
     };
-    if (K <= 128)
-      go(gate_kernel<T, 16, 8>, 16);
-    else if (K <= 256)
-      go(gate_kernel<T, 16, 16>, 16);
-    else if (K <= 1024)
-      go(gate_kernel<T, 64, 16>, 64);
-    else
-      go(gate_wide_kernel<T>, GATE_BLOCK);
-    TDC_CHECK_LAUNCH();
-    return 0;
+    return with_tail(K, Vec<T>::N, [&](auto tail) {
+      constexpr int TAIL = decltype(tail)::value;
+      if (K <= 128)
+        go(gate_kernel<T, 16, 8, TAIL>, 16);
+      else if (K <= 256)
+        go(gate_kernel<T, 16, 16, TAIL>, 16);
+      else if (K <= 1024)
+        go(gate_kernel<T, 64, 16, TAIL>, 64);
+      else
+        go(gate_wide_kernel<T>, GATE_BLOCK);
+      TDC_CHECK_LAUNCH();
+      return 0;
+    });
   });
 }
 
@@ -272,11 +279,14 @@ int tdc_topk_gate_bwd(int dtype, const void* scores, int64_t ld, const uint8_t* 
                          stream, (const T*)scores, ld, m, w, labels, stat, dw, n, K, k,
                          normalize != 0, (T*)ds);
     };
-    if (K <= 256)
-      go(gate_bwd_kernel<T, 16>, 16);
-    else
-      go(gate_bwd_kernel<T, 64>, 64);
-    TDC_CHECK_LAUNCH();
-    return 0;
+    return with_tail(K, Vec<T>::N, [&](auto tail) {
+      constexpr int TAIL = decltype(tail)::value;
+      if (K <= 256)
+        go(gate_bwd_kernel<T, 16, TAIL>, 16);
+      else
+        go(gate_bwd_kernel<T, 64, TAIL>, 64);
+      TDC_CHECK_LAUNCH();
+      return 0;
+    });
   });
 }

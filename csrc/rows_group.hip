@@ -217,108 +217,239 @@ __device__ __forceinline__ int kept_places(const int* offsets, int K, int64_t m)
   return t < 0 ? 0 : (t > m ? (int)m : t);
 }
 
-// A row's slots: L lanes read the row once and write it to each of its places (zeros at a
-// place behind the kept ones).
-template <typename T>
+// The three kernels below move rows of whole 16-byte vectors.  L lanes (a power of two up to
+// a wave) work on a row; a thread has U pieces of it in flight: U rows where a row is at
+// most L vectors, else (LONG) U vectors of one row, L apart, the rest of the row being the
+// next grid row's or pass's.  The last vector of a row that is no multiple is taken N
+// elements before the row's end: what overlaps is written twice with the same values.
+// Rows shorter than a vector (SHORT) go element by element.
+template <typename T, bool SHORT> __device__ __forceinline__ Raw16 take(const T* row, int c, int d) {
+  return RowVec<T, SHORT ? TAIL_SHORT : TAIL_NONE>::fetch(row, c, d);
+}
+template <typename T, bool SHORT>
+__device__ __forceinline__ void put(T* row, int c, int d, const Raw16& r) {
+  if constexpr (SHORT) {
+    T t[Vec<T>::N];
+    __builtin_memcpy(t, &r, 16);
+#pragma unroll
+    for (int i = 0; i < Vec<T>::N; ++i)
+      if (c + i < d) row[c + i] = t[i];
+  } else {
+    store16(row + min(c, d - Vec<T>::N), r);
+  }
+}
+
+// Row and column of a thread's piece u; false where there is none.
+template <int N, int U, bool LONG>
+__device__ __forceinline__ bool piece(int u, int L, int64_t n, int d, int pass, int64_t& row, int& c) {
+  const int lane = threadIdx.x & (L - 1), group = threadIdx.x / L, groups = 256 / L;
+  if (LONG) {
+    row = (int64_t)blockIdx.x * groups + group;
+    c = ((pass * U + u) * L + lane) * N;
+  } else {
+    row = ((int64_t)blockIdx.x * U + u) * groups + group;
+    c = lane * N;
+  }
+  return row < n && c < d;
+}
+
+// xg: every row is read once and written to the places of its k slots (zeros behind the
+// kept ones), J slots at a time: their places are all there before the first store, as a
+// wait for a load waits for the stores before it too (rows of 2 KiB with k = 8: @@ TB/s,
+// 3.5 with a place fetched before each store).
+template <typename T, int J, int U, bool LONG, bool SHORT>
 __global__ __launch_bounds__(256) void group_kernel(const T* __restrict__ x, int64_t ldx, int64_t n,
                                                     int k, int d, const int* __restrict__ offsets,
                                                     int K, const int* __restrict__ pos,
                                                     T* __restrict__ out, int L) {
-  constexpr int V = Vec<T>::N;
-  const int lane = threadIdx.x & (L - 1);
-  const int64_t row = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
-  if (row >= n) return;
+  constexpr int N = Vec<T>::N;
   const int kept = kept_places(offsets, K, n * k);
-  for (int c = lane * V; c < d; c += L * V) {
-    float v[V], zero[V];
-    load_vec<T>(x + row * ldx, c, d, v);
+  Raw16 v[U];
+  int64_t row[U];
+  int c[U];
+  bool in[U];
 #pragma unroll
-    for (int i = 0; i < V; ++i) zero[i] = 0.f;
-    for (int j = 0; j < k; ++j) {
-      const int p = pos[row * k + j];
-      if ((unsigned)p < (unsigned)(n * k)) {
-        if (p < kept)
-          store_vec<T>(out + (int64_t)p * d, c, d, v);
-        else
-          store_vec<T>(out + (int64_t)p * d, c, d, zero);
+  for (int u = 0; u < U; ++u) {
+    in[u] = piece<N, U, LONG>(u, L, n, d, blockIdx.y, row[u], c[u]);
+    v[u] = take<T, SHORT>(x + (in[u] ? row[u] : 0) * ldx, in[u] ? c[u] : 0, d);
+  }
+  for (int j0 = 0; j0 < k; j0 += J) {
+    int p[U][J];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        const int at = pos[(in[u] ? row[u] : 0) * k + min(j0 + j, k - 1)];
+        p[u][j] = in[u] && j0 + j < k ? at : -1;
       }
-    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+        if ((unsigned)p[u][j] < (unsigned)(n * k))
+          put<T, SHORT>(out + (int64_t)p[u][j] * d, c[u], d, if_kept(p[u][j] < kept, v[u]));
   }
 }
 
-// out[n] = sum_j w[n, j] y[pos[n, j]] (w null: 1).
 template <typename T>
+__device__ __forceinline__ float weight_at(const void* __restrict__ w, bool w32, int64_t slot) {
+  return w ? (w32 ? ((const float*)w)[slot] : up(((const T*)w)[slot])) : 1.f;
+}
+
+// out[n] = sum_j w[n, j] y[pos[n, j]] (w null: 1), J slots at a time.  A slot without a
+// place reads the row at place 0 (there is one) and drops it: the J * U loads have no
+// branch between them.
+template <typename T, int J, int U, bool LONG, bool SHORT>
 __global__ __launch_bounds__(256) void combine_kernel(const T* __restrict__ y, int64_t ldy, int64_t n,
                                                       int k, int d, const int* __restrict__ offsets,
                                                       int K, const int* __restrict__ pos,
                                                       const void* __restrict__ w, bool w32,
                                                       T* __restrict__ out, int L) {
-  constexpr int V = Vec<T>::N;
-  const int lane = threadIdx.x & (L - 1);
-  const int64_t row = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
-  if (row >= n) return;
+  constexpr int N = Vec<T>::N;
   const unsigned kept = (unsigned)kept_places(offsets, K, n * k);
-  for (int c = lane * V; c < d; c += L * V) {
-    float a[V];
+  int64_t row[U];
+  int c[U];
+  bool in[U];
+  float a[U][N];
 #pragma unroll
-    for (int i = 0; i < V; ++i) a[i] = 0.f;
-    for (int j = 0; j < k; ++j) {
-      const int64_t slot = row * k + j;
-      const unsigned p = (unsigned)pos[slot];
-      if (p < kept) {
-        const float wj = w ? (w32 ? ((const float*)w)[slot] : up(((const T*)w)[slot])) : 1.f;
-        float v[V];
-        load_vec<T>(y + (int64_t)p * ldy, c, d, v);
-#pragma unroll
-        for (int i = 0; i < V; ++i) a[i] = fmaf(wj, v[i], a[i]);
-      }
+  for (int u = 0; u < U; ++u) {
+    in[u] = piece<N, U, LONG>(u, L, n, d, blockIdx.y, row[u], c[u]);
+    if (!in[u]) {
+      row[u] = 0;
+      c[u] = 0;
     }
-    store_vec<T>(out + row * d, c, d, a);
+#pragma unroll
+    for (int i = 0; i < N; ++i) a[u][i] = 0.f;
   }
+  for (int j0 = 0; j0 < k; j0 += J) {
+    unsigned p[U][J];
+    float wj[U][J];
+    Raw16 v[U][J];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        const int64_t slot = row[u] * k + min(j0 + j, k - 1);
+        p[u][j] = j0 + j < k ? (unsigned)pos[slot] : kept;
+        wj[u][j] = weight_at<T>(w, w32, slot);
+      }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+        v[u][j] = take<T, SHORT>(y + (int64_t)(p[u][j] < kept ? p[u][j] : 0) * ldy, c[u], d);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        float f[N];
+        unpack<T>(v[u][j], f);
+        if (p[u][j] < kept)
+#pragma unroll
+          for (int i = 0; i < N; ++i) a[u][i] = fmaf(wj[u][j], f[i], a[u][i]);
+      }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (in[u]) put<T, SHORT>(out + row[u] * d, c[u], d, pack<T>(a[u]));
 }
 
-// Gradients of a slot: dy[p] = w dout[row], dw = <dout[row], y[p]>; either may be left out.
-template <typename T>
+// Gradients of a row's slots, J at a time: dy[p] = w dout[row], dw = <dout[row], y[p]>;
+// either may be left out (dy null, y null).  The row's passes and the sum over its lanes
+// are this thread group's, so dw needs no atomics.
+template <typename T, int J, int U, bool LONG, bool SHORT>
 __global__ __launch_bounds__(256) void combine_bwd_kernel(
     const T* __restrict__ dout, int64_t lddo, const T* __restrict__ y, int64_t ldy, int64_t n, int k,
     int d, const int* __restrict__ offsets, int K, const int* __restrict__ pos,
     const void* __restrict__ w, bool w32, T* __restrict__ dy, void* __restrict__ dw, int L) {
-  constexpr int V = Vec<T>::N;
+  constexpr int N = Vec<T>::N;
+  const unsigned m = (unsigned)(n * k);
+  const unsigned kept = (unsigned)kept_places(offsets, K, n * k);
   const int lane = threadIdx.x & (L - 1);
-  const int64_t slot = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
-  const int64_t m = n * k;
-  float dot = 0.f;
-  if (slot < m) {
-    const int64_t row = slot / k;
-    const unsigned kept = (unsigned)kept_places(offsets, K, m);
-    const unsigned p = (unsigned)pos[slot];
-    const float wj = w ? (w32 ? ((const float*)w)[slot] : up(((const T*)w)[slot])) : 1.f;
-    if (p < (unsigned)m)
-      for (int c = lane * V; c < d; c += L * V) {
-        float g[V], o[V];
+  const int passes = LONG ? (d + U * L * N - 1) / (U * L * N) : 1;
+  for (int j0 = 0; j0 < k; j0 += J) {
+    constexpr int S = LONG ? 1 : U;  // rows of a thread
+    float dot[S][J];
+    unsigned p[S][J];
+    float wj[S][J];
 #pragma unroll
-        for (int i = 0; i < V; ++i) o[i] = 0.f;
-        if (p < kept) {
-          load_vec<T>(dout + row * lddo, c, d, g);
-          if (dw) {
-            float v[V];
-            load_vec<T>(y + (int64_t)p * ldy, c, d, v);
+    for (int u = 0; u < S; ++u) {
+      int64_t row;
+      int c;
+      // every lane of the row takes its places, those without a column too
+      piece<N, U, LONG>(u, L, n, d, 0, row, c);
 #pragma unroll
-            for (int i = 0; i < V; ++i) dot = fmaf(g[i], v[i], dot);
-          }
-#pragma unroll
-          for (int i = 0; i < V; ++i) o[i] = wj * g[i];
-        }
-        if (dy) store_vec<T>(dy + (int64_t)p * d, c, d, o);
+      for (int j = 0; j < J; ++j) {
+        const int64_t slot = (row < n ? row : 0) * k + min(j0 + j, k - 1);
+        p[u][j] = row < n && j0 + j < k ? (unsigned)pos[slot] : m;
+        wj[u][j] = weight_at<T>(w, w32, slot);
+        dot[u][j] = 0.f;
       }
-  }
-  if (!dw) return;
-  for (int o = L / 2; o > 0; o >>= 1) dot += __shfl_xor(dot, o, 64);
-  if (slot < m && lane == 0) {
-    if (w32)
-      ((float*)dw)[slot] = dot;
-    else
-      ((T*)dw)[slot] = down<T>(dot);
+    }
+    for (int pass = 0; pass < passes; ++pass) {
+      int64_t row[U];
+      int c[U];
+      bool in[U];
+      Raw16 g[U], v[U][J];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        in[u] = piece<N, U, LONG>(u, L, n, d, pass, row[u], c[u]);
+        g[u] = take<T, SHORT>(dout + (in[u] ? row[u] : 0) * lddo, in[u] ? c[u] : 0, d);
+      }
+      if (y) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int j = 0; j < J; ++j) {
+            const unsigned at = p[LONG ? 0 : u][j];
+            v[u][j] = take<T, SHORT>(y + (int64_t)(at < kept ? at : 0) * ldy, in[u] ? c[u] : 0, d);
+          }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float f[N];
+        unpack<T>(g[u], f);
+        // elements that the vector before this one has counted already
+        const int twice = SHORT ? 0 : c[u] - min(c[u], d - N);
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+          const unsigned at = p[LONG ? 0 : u][j];
+          const float ww = wj[LONG ? 0 : u][j];
+          if (dy && in[u] && at < m) {
+            float o[N];
+#pragma unroll
+            for (int i = 0; i < N; ++i) o[i] = ww * f[i];
+            put<T, SHORT>(dy + (int64_t)at * d, c[u], d, if_kept(at < kept, pack<T>(o)));
+          }
+          if (y && in[u] && at < kept) {
+            float q[N];
+            unpack<T>(v[u][j], q);
+            float t = 0.f;
+#pragma unroll
+            for (int i = 0; i < N; ++i) t = fmaf(i >= twice ? f[i] : 0.f, i >= twice ? q[i] : 0.f, t);
+            dot[LONG ? 0 : u][j] += t;
+          }
+        }
+      }
+    }
+    if (!dw) continue;
+#pragma unroll
+    for (int u = 0; u < S; ++u) {
+      int64_t row;
+      int c;
+      piece<N, U, LONG>(u, L, n, d, 0, row, c);
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        float t = dot[u][j];
+        for (int o = L / 2; o > 0; o >>= 1) t += __shfl_xor(t, o, 64);
+        if (lane == 0 && row < n && j0 + j < k) {
+          if (w32)
+            ((float*)dw)[row * k + j0 + j] = t;
+          else
+            ((T*)dw)[row * k + j0 + j] = down<T>(t);
+        }
+      }
+    }
   }
 }
 
@@ -328,6 +459,33 @@ inline int lanes_for(int d, int v) {
   int l = 4;
   while (l < 64 && l < vecs) l *= 2;
   return l;
+}
+
+// f(LONG, SHORT) for rows of d elements in vectors of v.
+template <typename F> int with_rows(int d, int v, F&& f) {
+  if (d < v) return f(std::false_type(), std::true_type());
+  if (d > 64 * v) return f(std::true_type(), std::false_type());
+  return f(std::false_type(), std::false_type());
+}
+
+// Grid of U pieces per thread: rows, and (LONG) the passes over a row as grid rows.
+inline bool grid_for(int64_t n, int d, int v, int L, int U, bool is_long, bool passes, dim3& grid) {
+  const int64_t rows = (int64_t)(256 / L) * (is_long ? 1 : U);
+  const int64_t bx = (n + rows - 1) / rows;
+  const int by = is_long && passes ? (d + U * L * v - 1) / (U * L * v) : 1;
+  if (bx > 0x7fffffff || by > 65535) return false;
+  grid = dim3((unsigned)bx, (unsigned)by);
+  return true;
+}
+
+// f(J, U): slots at once and pieces of a thread, 8 to 16 loads in flight.
+template <typename F> int with_slots(int k, F&& f) {
+#define TDC_SLOTS(J, U) f(std::integral_constant<int, J>(), std::integral_constant<int, U>())
+  if (k == 1) return TDC_SLOTS(1, 4);
+  if (k == 2) return TDC_SLOTS(2, 4);
+  if (k <= 4) return TDC_SLOTS(4, 2);
+  return TDC_SLOTS(8, 2);
+#undef TDC_SLOTS
 }
 
 struct SortShape {
@@ -424,12 +582,20 @@ int tdc_group_rows(int dtype, const void* x, int64_t ldx, int64_t n, int k, int 
   if (n == 0) return 0;
   return with_type(dtype, [&](auto t) {
     using T = decltype(t);
-    const int L = lanes_for(d, Vec<T>::N);
-    const int64_t blocks = (n + 256 / L - 1) / (256 / L);
-    hipLaunchKernelGGL(group_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, stream, (const T*)x,
-                       ldx, n, k, d, offsets, K, pos, (T*)out, L);
-    TDC_CHECK_LAUNCH();
-    return 0;
+    constexpr int V = Vec<T>::N;
+    const int L = lanes_for(d, V);
+    return with_rows(d, V, [&](auto lng, auto shrt) {
+      return with_slots(k, [&](auto jj, auto uu) {
+        constexpr bool LONG = decltype(lng)::value, SHORT = decltype(shrt)::value;
+        constexpr int J = decltype(jj)::value, U = decltype(uu)::value;
+        dim3 grid;
+        if (!grid_for(n, d, V, L, U, LONG, true, grid)) return (int)hipErrorInvalidValue;
+        hipLaunchKernelGGL((group_kernel<T, J, U, LONG, SHORT>), grid, dim3(256), 0, stream,
+                           (const T*)x, ldx, n, k, d, offsets, K, pos, (T*)out, L);
+        TDC_CHECK_LAUNCH();
+        return 0;
+      });
+    });
   });
 }
 
@@ -439,12 +605,20 @@ int tdc_combine_rows(int dtype, const void* y, int64_t ldy, int64_t n, int k, in
   if (n == 0) return 0;
   return with_type(dtype, [&](auto t) {
     using T = decltype(t);
-    const int L = lanes_for(d, Vec<T>::N);
-    const int64_t blocks = (n + 256 / L - 1) / (256 / L);
-    hipLaunchKernelGGL(combine_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, stream, (const T*)y,
-                       ldy, n, k, d, offsets, K, pos, w, w32 != 0, (T*)out, L);
-    TDC_CHECK_LAUNCH();
-    return 0;
+    constexpr int V = Vec<T>::N;
+    const int L = lanes_for(d, V);
+    return with_rows(d, V, [&](auto lng, auto shrt) {
+      return with_slots(k, [&](auto jj, auto uu) {
+        constexpr bool LONG = decltype(lng)::value, SHORT = decltype(shrt)::value;
+        constexpr int J = decltype(jj)::value, U = decltype(uu)::value;
+        dim3 grid;
+        if (!grid_for(n, d, V, L, U, LONG, true, grid)) return (int)hipErrorInvalidValue;
+        hipLaunchKernelGGL((combine_kernel<T, J, U, LONG, SHORT>), grid, dim3(256), 0, stream,
+                           (const T*)y, ldy, n, k, d, offsets, K, pos, w, w32 != 0, (T*)out, L);
+        TDC_CHECK_LAUNCH();
+        return 0;
+      });
+    });
   });
 }
 
@@ -454,12 +628,20 @@ int tdc_combine_rows_bwd(int dtype, const void* dout, int64_t lddo, const void* 
   if (n == 0 || (!dy && !dw)) return 0;
   return with_type(dtype, [&](auto t) {
     using T = decltype(t);
-    const int L = lanes_for(d, Vec<T>::N);
-    const int64_t blocks = (n * k + 256 / L - 1) / (256 / L);
-    hipLaunchKernelGGL(combine_bwd_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, stream,
-                       (const T*)dout, lddo, (const T*)y, ldy, n, k, d, offsets, K, pos, w, w32 != 0,
-                       (T*)dy, dw, L);
-    TDC_CHECK_LAUNCH();
-    return 0;
+    constexpr int V = Vec<T>::N;
+    const int L = lanes_for(d, V);
+    return with_rows(d, V, [&](auto lng, auto shrt) {
+      return with_slots(k, [&](auto jj, auto uu) {
+        constexpr bool LONG = decltype(lng)::value, SHORT = decltype(shrt)::value;
+        constexpr int J = decltype(jj)::value, U = decltype(uu)::value;
+        dim3 grid;
+        if (!grid_for(n, d, V, L, U, LONG, false, grid)) return (int)hipErrorInvalidValue;
+        hipLaunchKernelGGL((combine_bwd_kernel<T, J, U, LONG, SHORT>), grid, dim3(256), 0, stream,
+                           (const T*)dout, lddo, (const T*)y, ldy, n, k, d, offsets, K, pos, w,
+                           w32 != 0, (T*)dy, dw, L);
+        TDC_CHECK_LAUNCH();
+        return 0;
+      });
+    });
   });
 }

@@ -23,18 +23,38 @@ constexpr int BLOCK = 256;
 
 template <int G> constexpr int block_of() { return G > BLOCK ? G : BLOCK; }
 
-template <typename T>
-__device__ __forceinline__ void load_weight(const void* __restrict__ w, bool w32, int c, int d,
-                                            float (&v)[Vec<T>::N]) {
-  if (w == nullptr) {
+// The weights of a vector of T: of its type, or N / 4 vectors of fp32.
+template <typename T, int TAIL> struct WeightVec {
+  static constexpr int N = Vec<T>::N;
+  // a row of d >= N elements of T has d >= 4: its fp32 weights never are short alone
+  using F = RowVec<float, TAIL>;
+  Raw16 r[N / 4];
+  __device__ __forceinline__ void fetch(const void* __restrict__ w, bool w32, int c, int d) {
+    if (w == nullptr) return;
+    if (w32) {
 #pragma unroll
-    for (int i = 0; i < Vec<T>::N; ++i) v[i] = 1.f;
-  } else if (w32) {
-    load_f32<Vec<T>::N>((const float*)w, c, d, v);
-  } else {
-    load_vec<T>((const T*)w, c, d, v);
+      for (int q = 0; q < N / 4; ++q) r[q] = F::fetch((const float*)w, c + 4 * q, d);
+    } else {
+      r[0] = RowVec<T, TAIL>::fetch((const T*)w, c, d);
+    }
   }
-}
+  __device__ __forceinline__ void value(const void* w, bool w32, int c, int d, float (&v)[N]) const {
+    if (w == nullptr) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = 1.f;
+    } else if (w32) {
+#pragma unroll
+      for (int q = 0; q < N / 4; ++q) {
+        float t[4];
+        F::value(r[q], c + 4 * q, d, t);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[4 * q + i] = t[i];
+      }
+    } else {
+      RowVec<T, TAIL>::value(r[0], c, d, v);
+    }
+  }
+};
 
 // N values of one lane to e4m3 with the exponent of their block of 32 columns (32 / N
 // neighbouring lanes).  The block's largest value lies in [2^7, 2^8) after the scaling:
@@ -63,40 +83,45 @@ __device__ __forceinline__ void store_fp8(uint8_t* __restrict__ q, uint8_t* __re
   if (c % 32 == 0) s[c / 32] = (uint8_t)(e + 127);
 }
 
-template <typename T, int G, int NV, bool FP8>
+template <typename T, int G, int NV, int TAIL, bool FP8>
 __global__ __launch_bounds__(block_of<G>()) void norm_kernel(
     const T* __restrict__ x, int64_t ldx, const T* __restrict__ r, int64_t ldr,
     const void* __restrict__ w, bool w32, int64_t n, int d, float eps, T* __restrict__ y,
     uint8_t* __restrict__ q, uint8_t* __restrict__ s, int dp, T* __restrict__ h,
     float* __restrict__ rstd) {
   constexpr int N = Vec<T>::N;
+  using R = RowVec<T, TAIL>;
   __shared__ float part[2][16];
   int turn = 0;
   const int lane = threadIdx.x % G;
   const int64_t row = (int64_t)blockIdx.x * (block_of<G>() / G) + threadIdx.x / G;
   if (row >= n) return;  // whole groups; G > 64: the block is one row of the grid
+  Raw16 xr[NV], rr[NV];
+  WeightVec<T, TAIL> wr[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) xr[i] = R::fetch(x + row * ldx, (i * G + lane) * N, d);
+  if (r) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) rr[i] = R::fetch(r + row * ldr, (i * G + lane) * N, d);
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i) wr[i].fetch(w, w32, (i * G + lane) * N, d);
   float v[NV][N];
   float sq = 0.f;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c = (i * G + lane) * N;
-    load_vec<T>(x + row * ldx, c, d, v[i]);
-  }
-  if (r) {
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (i * G + lane) * N;
+    R::value(xr[i], c, d, v[i]);
+    if (r) {
       float t[N];
-      load_vec<T>(r + row * ldr, c, d, t);
+      R::value(rr[i], c, d, t);
 #pragma unroll
       for (int j = 0; j < N; ++j) v[i][j] = up(down<T>(v[i][j] + t[j]));
-      store_vec<T>(h + row * d, c, d, v[i]);
+      R::store(h + row * d, c, d, v[i]);
     }
-  }
-#pragma unroll
-  for (int i = 0; i < NV; ++i)
 #pragma unroll
     for (int j = 0; j < N; ++j) sq = fmaf(v[i][j], v[i][j], sq);
+  }
   sq = group_sum<G>(sq, part, turn);
   const float rs = 1.f / sqrtf(sq / (float)d + eps);
   if (rstd && lane == 0) rstd[row] = rs;
@@ -104,7 +129,7 @@ __global__ __launch_bounds__(block_of<G>()) void norm_kernel(
   for (int i = 0; i < NV; ++i) {
     const int c = (i * G + lane) * N;
     float t[N];
-    load_weight<T>(w, w32, c, d, t);
+    wr[i].value(w, w32, c, d, t);
 #pragma unroll
     for (int j = 0; j < N; ++j) t[j] = v[i][j] * rs * t[j];
     if constexpr (FP8) {
@@ -113,7 +138,7 @@ __global__ __launch_bounds__(block_of<G>()) void norm_kernel(
       for (int j = 0; j < N; ++j) t[j] = c + j < d ? t[j] : 0.f;
       if (c < dp) store_fp8<N>(q + row * dp, s + row * (dp / 32), c, t);
     } else {
-      store_vec<T>(y + row * d, c, d, t);
+      R::store(y + row * d, c, d, t);
     }
   }
 }
@@ -121,37 +146,49 @@ __global__ __launch_bounds__(block_of<G>()) void norm_kernel(
 // The gradient.  A block goes over rows with a stride of the grid and keeps its share of dw
 // in registers; the shares of its row groups are added in LDS order and leave as one row of
 // `part`, which dw_kernel sums: no atomics, the same order in every run.
-template <typename T, int G, int NV>
+template <typename T, int G, int NV, int TAIL>
 __global__ __launch_bounds__(block_of<G>()) void norm_bwd_kernel(
     const T* __restrict__ h, int64_t ldh, const float* __restrict__ rstd, const void* __restrict__ w,
     bool w32, const T* __restrict__ dy, int64_t lddy, const T* __restrict__ dh, int64_t lddh,
     int64_t n, int d, T* __restrict__ dx, float* __restrict__ part) {
   constexpr int N = Vec<T>::N;
   constexpr int GROUPS = block_of<G>() / G;
+  using R = RowVec<T, TAIL>;
   __shared__ float sums[2][16];
   __shared__ float fold[GROUPS > 1 ? GROUPS : 1][GROUPS > 1 ? NV * G * N : 1];
   int turn = 0;
   const int lane = threadIdx.x % G, group = threadIdx.x / G;
   float dw[NV][N];
+  WeightVec<T, TAIL> wr[NV];
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
+  for (int i = 0; i < NV; ++i) {
+    wr[i].fetch(w, w32, (i * G + lane) * N, d);
 #pragma unroll
     for (int j = 0; j < N; ++j) dw[i][j] = 0.f;
+  }
   for (int64_t row = (int64_t)blockIdx.x * GROUPS + group; row < n;
        row += (int64_t)gridDim.x * GROUPS) {
     const float rs = rstd[row];
+    Raw16 hr[NV], gr[NV], er[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * G + lane) * N;
+      hr[i] = R::fetch(h + row * ldh, c, d);
+      gr[i] = R::fetch(dy + row * lddy, c, d);
+    }
+    if (dh) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) er[i] = R::fetch(dh + row * lddh, (i * G + lane) * N, d);
+    }
     float t[NV][N], g[NV][N];
     float dot = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * G + lane) * N;
-      load_vec<T>(h + row * ldh, c, d, t[i]);
-      load_vec<T>(dy + row * lddy, c, d, g[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
       float wv[N];
-      load_weight<T>(w, w32, (i * G + lane) * N, d, wv);
+      wr[i].value(w, w32, c, d, wv);
+      R::value(hr[i], c, d, t[i]);
+      R::value(gr[i], c, d, g[i]);
 #pragma unroll
       for (int j = 0; j < N; ++j) {
         t[i][j] *= rs;
@@ -169,11 +206,11 @@ __global__ __launch_bounds__(block_of<G>()) void norm_bwd_kernel(
       for (int j = 0; j < N; ++j) o[j] = rs * (g[i][j] - t[i][j] * c1);
       if (dh) {
         float e[N];
-        load_vec<T>(dh + row * lddh, c, d, e);
+        R::value(er[i], c, d, e);
 #pragma unroll
         for (int j = 0; j < N; ++j) o[j] += e[j];
       }
-      store_vec<T>(dx + row * d, c, d, o);
+      R::store(dx + row * d, c, d, o);
     }
   }
   if (!part) return;
@@ -200,60 +237,68 @@ __global__ __launch_bounds__(block_of<G>()) void norm_bwd_kernel(
   }
 }
 
-// dw[c] = sum of part[0..rows)[c]: a block takes 64 columns, its 16 waves every 16th row.
+// dw[c] = sum of part[0..rows)[c].  A block takes 16 columns (one 64-byte line of each
+// row), its 64 row groups every 64th row with 8 loads in flight each: 4 MiB of parts
+// (1024 x 1024) take @@ us, with 64 columns per block (16 blocks only) 20 us.
+constexpr int DW_COLS = 16, DW_ROWS = 64;
 template <typename W>
 __global__ __launch_bounds__(1024) void dw_kernel(const float* __restrict__ part, int rows, int d,
                                                   W* __restrict__ dw) {
-  __shared__ float s[16][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int c = blockIdx.x * 64 + lane;
+  __shared__ float s[DW_ROWS][DW_COLS + 1];
+  const int col = threadIdx.x % DW_COLS, group = threadIdx.x / DW_COLS;
+  const int c = blockIdx.x * DW_COLS + col;
   float a = 0.f;
-  if (c < d)
-    for (int k = wave; k < rows; k += 16) a += part[(int64_t)k * d + c];
-  s[wave][lane] = a;
+  if (c < d) {
+#pragma unroll 8
+    for (int k = group; k < rows; k += DW_ROWS) a += part[(int64_t)k * d + c];
+  }
+  s[group][col] = a;
   __syncthreads();
-  if (wave == 0 && c < d) {
+  // 64 groups to 4 by one thread per column and group, then to one
+  if (threadIdx.x < 4 * DW_COLS) {
     a = 0.f;
-    for (int k = 0; k < 16; ++k) a += s[k][lane];
-    dw[c] = down<W>(a);
+#pragma unroll
+    for (int k = 0; k < DW_ROWS / 4; ++k) a += s[group * (DW_ROWS / 4) + k][col];
+    a += __shfl_xor(a, 16, 64);
+    a += __shfl_xor(a, 32, 64);
+    if (group == 0 && c < d) dw[c] = down<W>(a);
   }
 }
 
-// q 2^e of 16 columns per thread.
-template <typename T>
+// q 2^e, one 16-byte vector of the result per thread, a row per grid row block: the reads
+// and writes of a wave are contiguous.  2^e is built from its bits (scale 0 is the subnormal
+// 2^-127), the product is exact.
+template <typename T, int TAIL>
 __global__ __launch_bounds__(BLOCK) void dequant_kernel(const uint8_t* __restrict__ q,
                                                         const uint8_t* __restrict__ s, int64_t n,
-                                                        int d, int dp, T* __restrict__ out) {
+                                                        int d, int dp, T* __restrict__ out,
+                                                        int rows) {
   constexpr int N = Vec<T>::N;
-  const int per = (d + 15) / 16;
-  const int64_t i = (int64_t)blockIdx.x * BLOCK + threadIdx.x;
-  const int64_t row = i / per;
-  const int c = (int)(i % per) * 16;
+  const int per = BLOCK / rows;  // threads of a row
+  const int64_t row = (int64_t)blockIdx.x * rows + threadIdx.x / per;
   if (row >= n) return;
-  const uint4 raw = *reinterpret_cast<const uint4*>(q + row * dp + c);
-  const int e = (int)s[row * (dp / 32) + c / 32] - 127;
-  const unsigned p[4] = {raw.x, raw.y, raw.z, raw.w};
-  float v[16];
+  for (int c = (threadIdx.x % per) * N; c < d; c += per * N) {
+    unsigned p[N / 4];
+    __builtin_memcpy(p, q + row * dp + c, N);
+    const unsigned e = s[row * (dp / 32) + c / 32];
+    const float f = __uint_as_float(e ? e << 23 : 0x00400000u);
+    float v[N];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    v[4 * k] = ldexpf(__builtin_amdgcn_cvt_f32_fp8((int)p[k], 0), e);
-    v[4 * k + 1] = ldexpf(__builtin_amdgcn_cvt_f32_fp8((int)p[k], 1), e);
-    v[4 * k + 2] = ldexpf(__builtin_amdgcn_cvt_f32_fp8((int)p[k], 2), e);
-    v[4 * k + 3] = ldexpf(__builtin_amdgcn_cvt_f32_fp8((int)p[k], 3), e);
-  }
-#pragma unroll
-  for (int k = 0; k < 16 / N; ++k) {
-    float t[N];
-#pragma unroll
-    for (int j = 0; j < N; ++j) t[j] = v[k * N + j];
-    if (c + k * N < d) store_vec<T>(out + row * d, c + k * N, d, t);
+    for (int k = 0; k < N / 4; ++k) {
+      v[4 * k] = __builtin_amdgcn_cvt_f32_fp8((int)p[k], 0) * f;
+      v[4 * k + 1] = __builtin_amdgcn_cvt_f32_fp8((int)p[k], 1) * f;
+      v[4 * k + 2] = __builtin_amdgcn_cvt_f32_fp8((int)p[k], 2) * f;
+      v[4 * k + 3] = __builtin_amdgcn_cvt_f32_fp8((int)p[k], 3) * f;
+    }
+    RowVec<T, TAIL>::store(out + row * d, c, d, v);
   }
 }
 
-// Calls f(G, NV) for a row of `vecs` vectors of 16 bytes: the fewest threads that hold it
+// Calls f(G, NV) for a row of `width` in vectors of N elements (16 bytes): the fewest threads that hold it
 // in at most 4 vectors each, a wave from 17 vectors on, so that the row's sum needs no
 // barrier up to 256 vectors (4 KiB).
-template <typename F> int with_shape(int vecs, F&& f) {
+template <int N, typename F> int with_shape(int width, F&& f) {
+  const int vecs = (width + N - 1) / N;
 #define TDC_SHAPE(G, NV) f(std::integral_constant<int, G>(), std::integral_constant<int, NV>())
   if (vecs <= 16) return TDC_SHAPE(16, 1);
   if (vecs <= 64) return TDC_SHAPE(64, 1);
@@ -262,7 +307,8 @@ template <typename F> int with_shape(int vecs, F&& f) {
   if (vecs <= 512) return TDC_SHAPE(256, 2);
   if (vecs <= 1024) return TDC_SHAPE(256, 4);
   if (vecs <= 2048) return TDC_SHAPE(1024, 2);
-  if (vecs <= 4096) return TDC_SHAPE(1024, 4);
+  if constexpr (N == 4)  // 16384 columns of fp32
+    if (vecs <= 4096) return TDC_SHAPE(1024, 4);
 #undef TDC_SHAPE
   return (int)hipErrorInvalidValue;
 }
@@ -279,7 +325,7 @@ int tdc_rms_norm(int dtype, const void* x, int64_t ldx, const void* r, int64_t l
   return with_type(dtype, [&](auto t) {
     using T = decltype(t);
     const int width = q ? dp : d;
-    return with_shape((width + Vec<T>::N - 1) / Vec<T>::N, [&](auto g, auto nv) {
+    return with_shape<Vec<T>::N>(width, [&](auto g, auto nv) {
       constexpr int G = decltype(g)::value, NV = decltype(nv)::value;
       constexpr int B = block_of<G>();
       const int64_t blocks = (n + B / G - 1) / (B / G);
@@ -289,12 +335,23 @@ int tdc_rms_norm(int dtype, const void* x, int64_t ldx, const void* r, int64_t l
                            (const T*)r, ldr, w, w32 != 0, n, d, eps, (T*)y, (uint8_t*)q,
                            (uint8_t*)s, dp, (T*)h, rstd);
       };
-      if (q)
-        go(norm_kernel<T, G, NV, true>);
-      else
-        go(norm_kernel<T, G, NV, false>);
-      TDC_CHECK_LAUNCH();
-      return 0;
+      return with_tail(d, Vec<T>::N, [&](auto tail) {
+        constexpr int TAIL = decltype(tail)::value;
+        // an fp8 row has 256 columns or more, and a row shorter than a vector few threads
+        if (q) {
+          if constexpr (G > 16 && (TAIL != TAIL_SHORT || (G == 64 && NV == 1)))
+            go(norm_kernel<T, G, NV, TAIL, true>);
+          else
+            return (int)hipErrorInvalidValue;
+        } else {
+          if constexpr (TAIL != TAIL_SHORT || G == 16)
+            go(norm_kernel<T, G, NV, TAIL, false>);
+          else
+            return (int)hipErrorInvalidValue;
+        }
+        TDC_CHECK_LAUNCH();
+        return 0;
+      });
     });
   });
 }
@@ -314,21 +371,25 @@ int tdc_rms_norm_bwd(int dtype, const void* h, int64_t ldh, const float* rstd, c
     using T = decltype(t);
     int used = 0;
     if (n > 0) {
-      const int rc = with_shape((d + Vec<T>::N - 1) / Vec<T>::N, [&](auto g, auto nv) {
+      const int rc = with_shape<Vec<T>::N>(d, [&](auto g, auto nv) {
         constexpr int G = decltype(g)::value, NV = decltype(nv)::value;
         constexpr int B = block_of<G>();
         const int64_t blocks = (n + B / G - 1) / (B / G);
         used = (int)(blocks < parts ? blocks : parts);
-        hipLaunchKernelGGL((norm_bwd_kernel<T, G, NV>), dim3(used), dim3(B), 0, stream,
-                           (const T*)h, ldh, rstd, w, w32 != 0, (const T*)dy, lddy, (const T*)dh,
-                           lddh, n, d, (T*)dx, dw ? part : nullptr);
-        TDC_CHECK_LAUNCH();
-        return 0;
+        return with_tail(d, Vec<T>::N, [&](auto tail) {
+          constexpr int TAIL = decltype(tail)::value;
+          if constexpr (TAIL != TAIL_SHORT || G == 16)
+            hipLaunchKernelGGL((norm_bwd_kernel<T, G, NV, TAIL>), dim3(used), dim3(B), 0, stream,
+                               (const T*)h, ldh, rstd, w, w32 != 0, (const T*)dy, lddy, (const T*)dh,
+                               lddh, n, d, (T*)dx, dw ? part : nullptr);
+          TDC_CHECK_LAUNCH();
+          return 0;
+        });
       });
       if (rc) return rc;
     }
     if (dw) {
-      const dim3 grid((unsigned)((d + 63) / 64));
+      const dim3 grid((unsigned)((d + DW_COLS - 1) / DW_COLS));
       if (w32)
         hipLaunchKernelGGL(dw_kernel<float>, grid, dim3(1024), 0, stream, part, used, d, (float*)dw);
       else
@@ -343,13 +404,20 @@ int tdc_dequant_fp8(int dtype, const void* q, const void* s, int64_t n, int d, i
                     hipStream_t stream) {
   if (n == 0) return 0;
   if (dp % 32 != 0 || d > dp) return (int)hipErrorInvalidValue;
-  const int64_t blocks = (n * ((d + 15) / 16) + BLOCK - 1) / BLOCK;
-  if (blocks > 0x7fffffff) return (int)hipErrorInvalidValue;
   return with_type(dtype, [&](auto t) {
     using T = decltype(t);
-    hipLaunchKernelGGL(dequant_kernel<T>, dim3((unsigned)blocks), dim3(BLOCK), 0, stream,
-                       (const uint8_t*)q, (const uint8_t*)s, n, d, dp, (T*)out);
-    TDC_CHECK_LAUNCH();
-    return 0;
+    // rows of a block: as many as its threads cover once
+    const int vecs = (d + Vec<T>::N - 1) / Vec<T>::N;
+    int rows = 1;
+    while (rows < 32 && rows * 2 * vecs <= BLOCK) rows *= 2;
+    const int64_t blocks = (n + rows - 1) / rows;
+    if (blocks > 0x7fffffff) return (int)hipErrorInvalidValue;
+    return with_tail(d, Vec<T>::N, [&](auto tail) {
+      constexpr int TAIL = decltype(tail)::value;
+      hipLaunchKernelGGL((dequant_kernel<T, TAIL>), dim3((unsigned)blocks), dim3(BLOCK), 0, stream,
+                         (const uint8_t*)q, (const uint8_t*)s, n, d, dp, (T*)out, rows);
+      TDC_CHECK_LAUNCH();
+      return 0;
+    });
   });
 }
