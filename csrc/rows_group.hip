@@ -4,8 +4,8 @@
 //   order[p] = slot at place p, pos[slot] = p, offsets[c] .. offsets[c + 1] = the places of
 //   cluster c.  Slots whose label is not in [0, K) come after offsets[K], in slot order.
 // The sort goes by digits of at most 11 bits: one pass up to K = 2047, two up to 2^22 - 1.
-// A pass counts its digits per chunk of 4096 slots, sums the counts over the chunks and
-// scatters; ranks inside a chunk come from ballots, so that equal labels keep their order
+// A pass counts its digits per chunk of 1024 to 4096 slots, sums the counts over the chunks
+// and scatters; ranks inside a chunk come from ballots, so that equal labels keep their order
 // and every run gives the same plan (no atomics on positions).
 //
 //   group:    xg[p] = x[order[p] / k]          gradient: dx[n] = sum_j dxg[pos[n, j]]
@@ -20,10 +20,11 @@ namespace rows {
 
 constexpr int SORT_BLOCK = 256;
 constexpr int SORT_WAVES = SORT_BLOCK / 64;
-constexpr int SORT_PER_LANE = 16;
-constexpr int SORT_CHUNK = SORT_BLOCK * SORT_PER_LANE;
 constexpr int DIGIT_BITS = 11;
 constexpr int MAX_DIGITS = 1 << DIGIT_BITS;
+// Chunks whose counts every block sums itself; above, a kernel of its own does (131072
+// labels of 257 keys: 16 us in two launches, 30 in three).
+constexpr int DIRECT_CHUNKS = 64;
 
 // The sort key of a slot: its label, or K where that is none of the clusters.
 template <typename I> __device__ __forceinline__ int key_of(const I* labels, int64_t i, int K) {
@@ -44,21 +45,33 @@ struct FromPairs {
   __device__ __forceinline__ int slot(int64_t i) const { return pairs[i].y; }
 };
 
-template <typename In>
+// The keys of a wave's 64 * PER slots, -1 past the end; the loads go out together.
+template <int PER, typename In>
+__device__ __forceinline__ void load_keys(const In& in, int64_t at, int64_t m, int (&key)[PER]) {
+#pragma unroll
+  for (int i = 0; i < PER; ++i) key[i] = in.key(min(at + i * 64, m - 1));
+#pragma unroll
+  for (int i = 0; i < PER; ++i) key[i] = at + i * 64 < m ? key[i] : -1;
+}
+
+// hist[digit * ds + chunk * cs] = slots of the chunk with that digit
+template <typename In, int PER>
 __global__ __launch_bounds__(SORT_BLOCK) void sort_count_kernel(In in, int64_t m, int shift,
-                                                                int digits, int* __restrict__ hist) {
+                                                                int bits, int digits,
+                                                                int* __restrict__ hist,
+                                                                int64_t ds, int64_t cs) {
   __shared__ int cnt[MAX_DIGITS];
+  const int mask = (1 << bits) - 1;
+  int key[PER];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  load_keys<PER>(in, (int64_t)blockIdx.x * (SORT_BLOCK * PER) + wave * (64 * PER) + lane, m, key);
   for (int d = threadIdx.x; d < digits; d += SORT_BLOCK) cnt[d] = 0;
   __syncthreads();
-  const int64_t base = (int64_t)blockIdx.x * SORT_CHUNK;
 #pragma unroll
-  for (int i = 0; i < SORT_PER_LANE; ++i) {
-    const int64_t at = base + i * SORT_BLOCK + threadIdx.x;
-    if (at < m) atomicAdd(&cnt[(in.key(at) >> shift) & (MAX_DIGITS - 1)], 1);
-  }
+  for (int i = 0; i < PER; ++i)
+    if (key[i] >= 0) atomicAdd(&cnt[(key[i] >> shift) & mask], 1);
   __syncthreads();
-  for (int d = threadIdx.x; d < digits; d += SORT_BLOCK)
-    hist[(int64_t)d * gridDim.x + blockIdx.x] = cnt[d];
+  for (int d = threadIdx.x; d < digits; d += SORT_BLOCK) hist[d * ds + blockIdx.x * cs] = cnt[d];
 }
 
 // Exclusive sum over the 256 threads of a block; total: the whole sum.
@@ -100,69 +113,97 @@ __global__ __launch_bounds__(SORT_BLOCK) void sort_scan_kernel(int* __restrict__
   if (threadIdx.x == 0) totals[blockIdx.x] = run;
 }
 
-// Places of a chunk's slots.  With one chunk (hist == null) the block's own counts are the
-// totals, and the whole sort is this launch.
-template <typename In, bool LAST>
+// Places of a chunk's slots.  One chunk: its own counts are the totals, and the whole sort
+// is this launch.  A few: every block sums the counts hist[chunk][digit].  Many (totals):
+// sort_scan_kernel has summed hist[digit][chunk].
+template <typename In, int PER, bool LAST>
 __global__ __launch_bounds__(SORT_BLOCK) void sort_scatter_kernel(
     In in, int64_t m, int shift, int digits, int bits, const int* __restrict__ hist,
     const int* __restrict__ totals, int2* __restrict__ pairs, int* __restrict__ keys,
     int* __restrict__ order, int* __restrict__ pos, int* __restrict__ offsets) {
   __shared__ int cnt[SORT_WAVES][MAX_DIGITS];
+  __shared__ int s_total[MAX_DIGITS], s_before[MAX_DIGITS];
   __shared__ int s_wave[SORT_WAVES];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  for (int d = threadIdx.x; d < digits; d += SORT_BLOCK)
+  const int chunk = blockIdx.x, chunks = gridDim.x, mask = (1 << bits) - 1;
+  // a wave owns 64 * PER slots in a row, 64 of them at a time
+  const int64_t first = (int64_t)chunk * (SORT_BLOCK * PER) + wave * (64 * PER);
+  int key[PER];
+  if (m > 0) load_keys<PER>(in, first + lane, m, key);
+  for (int d = threadIdx.x; d < digits; d += SORT_BLOCK) {
 #pragma unroll
     for (int i = 0; i < SORT_WAVES; ++i) cnt[i][d] = 0;
-  __syncthreads();
-  // a wave owns 1024 slots in a row, 64 of them at a time
-  const int64_t base = (int64_t)blockIdx.x * SORT_CHUNK + wave * (64 * SORT_PER_LANE) + lane;
-  int key[SORT_PER_LANE];
-#pragma unroll
-  for (int i = 0; i < SORT_PER_LANE; ++i) {
-    const int64_t at = base + i * 64;
-    key[i] = at < m ? in.key(at) : -1;
-    if (at < m) atomicAdd(&cnt[wave][(key[i] >> shift) & (MAX_DIGITS - 1)], 1);
+    s_total[d] = 0;
+    s_before[d] = 0;
   }
   __syncthreads();
-  // first place of each digit, then of each wave's part of it: 8 digits per thread
-  constexpr int PER = MAX_DIGITS / SORT_BLOCK;
-  int sum = 0, have[PER];
+  if (m > 0) {
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int d = threadIdx.x * PER + i;
-    int t = 0;
-    if (d < digits) {
-      if (totals) {
-        t = totals[d];
-      } else {
-        for (int q = 0; q < SORT_WAVES; ++q) t += cnt[q][d];
-      }
+    for (int i = 0; i < PER; ++i)
+      if (key[i] >= 0) atomicAdd(&cnt[wave][(key[i] >> shift) & mask], 1);
+  }
+  if (totals) {
+    for (int d = threadIdx.x; d < digits; d += SORT_BLOCK) {
+      s_total[d] = totals[d];
+      s_before[d] = hist[(int64_t)d * chunks + chunk];
     }
-    have[i] = t;
-    sum += t;
+  } else if (chunks > 1) {
+    // each wave a quarter of the chunks, all of a digit's loads in flight
+    constexpr int PART = DIRECT_CHUNKS / SORT_WAVES;
+    for (int d = lane; d < digits; d += 64) {
+      int v[PART], t = 0, before = 0;
+#pragma unroll
+      for (int i = 0; i < PART; ++i)
+        v[i] = hist[min(wave * PART + i, chunks - 1) * digits + d];
+#pragma unroll
+      for (int i = 0; i < PART; ++i) {
+        const int c = wave * PART + i;
+        t += c < chunks ? v[i] : 0;
+        before += c < chunk ? v[i] : 0;
+      }
+      atomicAdd(&s_total[d], t);
+      atomicAdd(&s_before[d], before);
+    }
+  }
+  __syncthreads();
+  // first place of each digit, then of each wave's part of it
+  const int own = (digits + SORT_BLOCK - 1) / SORT_BLOCK;  // digits of a thread, in a row
+  int sum = 0;
+  for (int i = 0; i < own; ++i) {
+    const int d = threadIdx.x * own + i;
+    if (d < digits) {
+      if (chunks == 1) {
+        int t = 0;
+#pragma unroll
+        for (int q = 0; q < SORT_WAVES; ++q) t += cnt[q][d];
+        s_total[d] = t;
+      }
+      sum += s_total[d];
+    }
   }
   int total;
-  int first = block_scan(sum, s_wave, total);
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int d = threadIdx.x * PER + i;
+  int at = block_scan(sum, s_wave, total);
+  for (int i = 0; i < own; ++i) {
+    const int d = threadIdx.x * own + i;
     if (d < digits) {
-      if (offsets && blockIdx.x == 0) offsets[d] = first;
-      int at = first + (hist ? hist[(int64_t)d * gridDim.x + blockIdx.x] : 0);
+      if (offsets && chunk == 0) offsets[d] = at;
+      int next = at + s_before[d];
+#pragma unroll
       for (int q = 0; q < SORT_WAVES; ++q) {
         const int c = cnt[q][d];
-        cnt[q][d] = at;
-        at += c;
+        cnt[q][d] = next;
+        next += c;
       }
+      at += s_total[d];
     }
-    first += have[i];
   }
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < SORT_PER_LANE; ++i) {
-    const int64_t at = base + i * 64;
-    const bool in_range = at < m;
-    const int d = in_range ? (key[i] >> shift) & (MAX_DIGITS - 1) : 0;
+  for (int i = 0; i < PER; ++i) {
+    if (first + i * 64 >= m) break;  // the same for the wave
+    const int64_t slot_at = first + i * 64 + lane;
+    const bool in_range = slot_at < m;
+    const int d = in_range ? (key[i] >> shift) & mask : 0;
     // lanes with the same digit as this one
     unsigned long long same = __ballot(in_range);
     for (int b = 0; b < bits; ++b) {
@@ -176,26 +217,31 @@ __global__ __launch_bounds__(SORT_BLOCK) void sort_scatter_kernel(
       // the last lane of the digit moves its next place on, after all have read it
       __builtin_amdgcn_wave_barrier();
       if ((same >> lane) == 1ull) *next = p + 1;
+      pos[slot_at] = p;  // of what stood here before the pass
       if constexpr (LAST) {
-        const int slot = in.slot(at);
-        order[p] = slot;
-        pos[slot] = p;
+        order[p] = in.slot(slot_at);
         if (keys) keys[p] = key[i];
       } else {
-        pairs[p] = make_int2(key[i], in.slot(at));
+        pairs[p] = make_int2(key[i], in.slot(slot_at));
       }
     }
     __builtin_amdgcn_wave_barrier();
   }
 }
 
+// The end of a sort in two passes.  pos[slot] holds the place after the first pass, `moved`
+// where the second put what stood there: the slot's place is read through both (1M labels:
+// 18 us for the second pass and 11 here; 31 and 5 where that pass wrote pos[slot] itself, 4
+// bytes at a time all over).
 // offsets[c] = first place whose key is c or more, for c in 0..K: the places where the key
 // steps up write those they step over, a whole wave at a time.
-__global__ __launch_bounds__(SORT_BLOCK) void sort_offsets_kernel(const int* __restrict__ keys,
-                                                                  int m, int K,
-                                                                  int* __restrict__ offsets) {
+__global__ __launch_bounds__(SORT_BLOCK) void sort_finish_kernel(const int* __restrict__ keys,
+                                                                 const int* __restrict__ moved,
+                                                                 int m, int K, int* __restrict__ pos,
+                                                                 int* __restrict__ offsets) {
   const int lane = threadIdx.x & 63;
   const int64_t p = (int64_t)blockIdx.x * SORT_BLOCK + threadIdx.x;
+  if (p < m) pos[p] = moved[pos[p]];
   int lo = 0, hi = 0;  // this place writes offsets lo .. hi - 1
   if (p <= m) {
     lo = p == 0 ? 0 : keys[p - 1] + 1;
@@ -255,7 +301,7 @@ __device__ __forceinline__ bool piece(int u, int L, int64_t n, int d, int pass, 
 
 // xg: every row is read once and written to the places of its k slots (zeros behind the
 // kept ones), J slots at a time: their places are all there before the first store, as a
-// wait for a load waits for the stores before it too (rows of 2 KiB with k = 8: @@ TB/s,
+// wait for a load waits for the stores before it too (rows of 2 KiB with k = 8: 6.4 TB/s,
 // 3.5 with a place fetched before each store).
 template <typename T, int J, int U, bool LONG, bool SHORT>
 __global__ __launch_bounds__(256) void group_kernel(const T* __restrict__ x, int64_t ldx, int64_t n,
@@ -489,92 +535,90 @@ template <typename F> int with_slots(int k, F&& f) {
 }
 
 struct SortShape {
-  int64_t m;
-  int bits, low, high;  // digits of the first and the second pass (0: one pass)
+  int low, high;  // bits of the first and the second pass's digit (0: one pass)
+  int per;        // slots per thread: the fewest that leave DIRECT_CHUNKS chunks, up to 16
   int64_t chunks;
+  int digits[2];
+
+  SortShape(int64_t m, int K) {
+    int bits = 1;
+    while ((K >> bits) != 0) ++bits;  // keys 0..K
+    low = bits <= DIGIT_BITS ? bits : (bits + 1) / 2;
+    high = bits - low;
+    per = 4;
+    // one block sorts up to 4096 alone
+    while (per < 16 && (m > (int64_t)SORT_BLOCK * per * DIRECT_CHUNKS || m <= SORT_BLOCK * 16)) per *= 2;
+    chunks = std::max<int64_t>(1, (m + SORT_BLOCK * per - 1) / (SORT_BLOCK * per));
+    digits[0] = high ? 1 << low : K + 1;
+    digits[1] = high ? (K >> low) + 1 : 0;
+  }
+  int64_t most() const { return std::max(digits[0], digits[1]); }
+  // counts of a pass, totals behind them, to whole int2
+  int64_t count_words() const {
+    return chunks == 1 ? 0 : (most() * (chunks + (chunks > DIRECT_CHUNKS ? 1 : 0)) + 1) / 2 * 2;
+  }
 };
-
-inline SortShape sort_shape(int64_t m, int K) {
-  SortShape s;
-  s.m = m;
-  s.bits = 1;
-  while ((K >> s.bits) != 0) ++s.bits;  // keys 0..K
-  s.low = s.bits <= DIGIT_BITS ? s.bits : DIGIT_BITS;
-  s.high = s.bits - s.low;
-  s.chunks = (m + SORT_CHUNK - 1) / SORT_CHUNK;
-  return s;
-}
-
-inline int digits_of(const SortShape& s, int pass, int K) {
-  if (s.high == 0) return K + 1;
-  return pass == 0 ? 1 << s.low : (K >> s.low) + 1;
-}
 
 }  // namespace rows
 }  // namespace tdc
 
 using namespace tdc::rows;
 
-// int32 words of scratch of a plan (counts, totals and, with two passes, pairs and keys).
+// int32 words of scratch of a plan (counts, totals and, with two passes, pairs, keys and moves).
 int64_t tdc_group_plan_work(int64_t m, int K) {
-  if (m <= 0) return 0;
-  const SortShape s = sort_shape(m, K);
-  const int64_t digits = std::max(digits_of(s, 0, K), s.high ? digits_of(s, 1, K) : 0);
-  int64_t words = s.chunks > 1 ? digits * (s.chunks + 1) : 0;
-  words += words & 1;  // the pairs are 8-byte aligned
-  if (s.high) words += 3 * m;
-  return words;
+  const SortShape s(m, K);
+  return s.count_words() + (s.high ? 4 * m : 0);
 }
 
 int tdc_group_plan(int wide_labels, const void* labels, int64_t m, int K, int* work, int* order,
                    int* pos, int* offsets, hipStream_t stream) {
   if (K < 1 || K >= (1 << 22) || m < 0 || m > 0x7ffffffe) return (int)hipErrorInvalidValue;
-  const SortShape s = sort_shape(m, K);
-  const int most = std::max(digits_of(s, 0, K), s.high ? digits_of(s, 1, K) : 0);
-  int* hist = nullptr;
-  int* totals = nullptr;
-  int64_t used = 0;
-  if (s.chunks > 1) {
-    hist = work;
-    totals = work + (int64_t)most * s.chunks;
-    used = (int64_t)most * (s.chunks + 1);
-    used += used & 1;
-  }
-  int2* pairs = s.high ? reinterpret_cast<int2*>(work + used) : nullptr;
-  int* keys = s.high ? work + used + 2 * m : nullptr;
-  const dim3 grid((unsigned)std::max<int64_t>(s.chunks, 1)), block(SORT_BLOCK);
-  auto pass = [&](auto in, auto last, int shift, int bits, int digits) {
+  const SortShape s(m, K);
+  int* hist = s.chunks > 1 ? work : nullptr;
+  int* totals = s.chunks > DIRECT_CHUNKS ? work + s.most() * s.chunks : nullptr;
+  int2* pairs = s.high ? reinterpret_cast<int2*>(work + s.count_words()) : nullptr;
+  int* keys = s.high ? work + s.count_words() + 2 * m : nullptr;
+  int* moved = s.high ? keys + m : nullptr;
+  const dim3 grid((unsigned)s.chunks), block(SORT_BLOCK);
+  auto pass = [&](auto in, auto last, auto per, int shift, int bits, int digits) {
     constexpr bool LAST = decltype(last)::value;
+    constexpr int PER = decltype(per)::value;
     using In = decltype(in);
-    if (s.chunks > 1) {
-      hipLaunchKernelGGL(sort_count_kernel<In>, grid, block, 0, stream, in, m, shift, digits, hist);
+    if (hist) {
+      hipLaunchKernelGGL((sort_count_kernel<In, PER>), grid, block, 0, stream, in, m, shift, bits,
+                         digits, hist, totals ? s.chunks : 1, totals ? 1 : (int64_t)digits);
       TDC_CHECK_LAUNCH();
+    }
+    if (totals) {
       hipLaunchKernelGGL(sort_scan_kernel, dim3(digits), block, 0, stream, hist, (int)s.chunks,
                          totals);
       TDC_CHECK_LAUNCH();
     }
-    hipLaunchKernelGGL((sort_scatter_kernel<In, LAST>), grid, block, 0, stream, in, m, shift, digits,
-                       bits, hist, totals, pairs, LAST ? keys : nullptr, order, pos,
-                       s.high ? nullptr : offsets);
+    hipLaunchKernelGGL((sort_scatter_kernel<In, PER, LAST>), grid, block, 0, stream, in, m, shift,
+                       digits, bits, hist, totals, pairs, LAST ? keys : nullptr, order,
+                       LAST && s.high ? moved : pos, s.high ? nullptr : offsets);
     TDC_CHECK_LAUNCH();
     return 0;
   };
-  auto all = [&](auto in) {
-    if (s.high == 0) return pass(in, std::true_type(), 0, s.low, digits_of(s, 0, K));
-    int rc = 0;
+  auto all = [&](auto in, auto per) {
+    if (s.high == 0) return pass(in, std::true_type(), per, 0, s.low, s.digits[0]);
     if (m > 0) {
-      rc = pass(in, std::false_type(), 0, s.low, digits_of(s, 0, K));
-      if (rc == 0)
-        rc = pass(FromPairs{pairs}, std::true_type(), s.low, s.high, digits_of(s, 1, K));
+      int rc = pass(in, std::false_type(), per, 0, s.low, s.digits[0]);
+      if (rc == 0) rc = pass(FromPairs{pairs}, std::true_type(), per, s.low, s.high, s.digits[1]);
+      if (rc) return rc;
     }
-    if (rc) return rc;
-    hipLaunchKernelGGL(sort_offsets_kernel, dim3((unsigned)((m + 1 + SORT_BLOCK - 1) / SORT_BLOCK)),
-                       block, 0, stream, keys, (int)m, K, offsets);
+    hipLaunchKernelGGL(sort_finish_kernel, dim3((unsigned)((m + 1 + SORT_BLOCK - 1) / SORT_BLOCK)),
+                       block, 0, stream, keys, moved, (int)m, K, pos, offsets);
     TDC_CHECK_LAUNCH();
     return 0;
   };
-  if (wide_labels) return all(FromLabels<int64_t>{(const int64_t*)labels, K});
-  return all(FromLabels<int32_t>{(const int32_t*)labels, K});
+  auto with_per = [&](auto in) {
+    if (s.per == 4) return all(in, std::integral_constant<int, 4>());
+    if (s.per == 8) return all(in, std::integral_constant<int, 8>());
+    return all(in, std::integral_constant<int, 16>());
+  };
+  if (wide_labels) return with_per(FromLabels<int64_t>{(const int64_t*)labels, K});
+  return with_per(FromLabels<int32_t>{(const int32_t*)labels, K});
 }
 
 int tdc_group_rows(int dtype, const void* x, int64_t ldx, int64_t n, int k, int d,
