@@ -6,8 +6,17 @@
 //   not normalize: w = softmax over all allowed p, at the chosen;
 //                  ds_i = p_i (dw_i [chosen] - sum w dw)
 //
-// Scores are compared as 32-bit whole numbers of the same order (0 = not to be chosen), so
-// the choice does not depend on any rounding; exp and the sums are fp32.
+// Scores are compared as whole numbers of the same order (0 = not to be chosen), so the
+// choice does not depend on any rounding; exp and the sums are fp32.
+//
+// Up to 4096 clusters a row stays in the registers of L threads, 16 scores each.  A score
+// and its index become one number, the index in place of the score's last 7 to 12 bits as
+// fp32: 16-bit types have nothing there.  The j-th choice is the largest number
+// below the (j-1)-th, found as the smallest of (limit - number), where what is above the
+// limit wraps around to more than the rest: 1.5 instructions per score and round, nothing
+// is taken out.  Where fp32 loses bits that are not zero and two neighbours among the first
+// k + 1 choices agree in the bits that are left, the rows of that wave are chosen again by
+// the whole scores.  65536 x 256 fp32, k = 8: @@ us, 37 with whole scores in every round.
 #include "rows_common.h"
 
 namespace tdc {
@@ -38,83 +47,200 @@ struct Mask {
   }
 };
 
-// L lanes work on a row, each with R scores in registers.  Every round takes the largest
-// that is left, over the registers and then over the lanes.
-template <typename T, int L, int R, int TAIL>
+// The mask of a vector of N scores: bit i of bits() is element c + i's.  Neighbouring bytes
+// are one load, taken N bytes before the row's end for its last, partial vector.
+template <int N, int TAIL> struct MaskVec {
+  uint64_t r;
+  __device__ __forceinline__ void fetch(const Mask& m, int64_t row, int c, int K) {
+    r = ~0ull;
+    if (m.p == nullptr) return;
+    if (TAIL != TAIL_SHORT && m.cs == 1) {
+      r = 0;
+      __builtin_memcpy(&r, m.p + row * m.rs + min(c, K - N), N);
+    }
+  }
+  __device__ __forceinline__ unsigned bits(const Mask& m, int64_t row, int c, int K) const {
+    unsigned in = 0;
+    if (m.p != nullptr && (TAIL == TAIL_SHORT || m.cs != 1)) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) in |= (c + i < K && m.at(row, c + i)) ? 1u << i : 0u;
+      return in;
+    }
+    uint64_t v = r;
+    if (m.p != nullptr && TAIL == TAIL_SHIFT) v >>= 8 * min(c - min(c, K - N), N - 1);
+#pragma unroll
+    for (int i = 0; i < N; ++i) in |= (c + i < K && (v >> (8 * i) & 0xff)) ? 1u << i : 0u;
+    return in;
+  }
+};
+
+// Over the L threads of a row, the result in each: rotations within 16 lanes, the four rows
+// of a wave through scalars, the waves of a block through LDS (two rows in turn, one
+// barrier).
+template <int CTRL> __device__ __forceinline__ unsigned rotated(unsigned v) {
+  return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
+}
+template <typename Op> __device__ __forceinline__ unsigned row_all(unsigned v, Op op) {
+  v = op(v, rotated<0x128>(v));
+  v = op(v, rotated<0x124>(v));
+  v = op(v, rotated<0x122>(v));
+  return op(v, rotated<0x121>(v));
+}
+template <int L, typename Op>
+__device__ __forceinline__ unsigned group_all(unsigned v, Op op, unsigned (*s)[4], int& turn) {
+  v = row_all(v, op);
+  if constexpr (L > 16) {
+    v = op(op((unsigned)__builtin_amdgcn_readlane((int)v, 0),
+              (unsigned)__builtin_amdgcn_readlane((int)v, 16)),
+           op((unsigned)__builtin_amdgcn_readlane((int)v, 32),
+              (unsigned)__builtin_amdgcn_readlane((int)v, 48)));
+  }
+  if constexpr (L > 64) {
+    unsigned* p = s[turn];
+    turn ^= 1;
+    if ((threadIdx.x & 63) == 0) p[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = op(op(p[0], p[1]), op(p[2], p[3]));
+  }
+  return v;
+}
+struct Least {
+  __device__ __forceinline__ unsigned operator()(unsigned a, unsigned b) const { return min(a, b); }
+};
+struct Most {
+  __device__ __forceinline__ unsigned operator()(unsigned a, unsigned b) const { return max(a, b); }
+};
+struct Any {
+  __device__ __forceinline__ unsigned operator()(unsigned a, unsigned b) const { return a | b; }
+};
+struct Sum {
+  __device__ __forceinline__ unsigned operator()(unsigned a, unsigned b) const {
+    return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+  }
+};
+
+template <int R> constexpr int column(int i, int v, int L, int lane) {
+  return ((i / v) * L + lane) * v + i % v;
+}
+
+template <typename T, int L, int R, int TAIL, bool MASKED>
 __global__ __launch_bounds__(GATE_BLOCK) void gate_kernel(const T* __restrict__ scores, int64_t ld,
                                                           Mask mask, int64_t n, int K, int k,
                                                           bool normalize, float* __restrict__ w,
                                                           int* __restrict__ labels,
                                                           float* __restrict__ stat) {
   constexpr int V = Vec<T>::N;
+  constexpr unsigned INDEX = L * R - 1;       // the bits of a column
+  constexpr unsigned NONE = 0x007fffffu;      // the place of -inf: it and less is not chosen
+  __shared__ unsigned s_all[2][4];
+  int turn = 0;
   const int lane = threadIdx.x % L;
   const int64_t row = (int64_t)blockIdx.x * (GATE_BLOCK / L) + threadIdx.x / L;
-  if (row >= n) return;
-  unsigned key[R];
-  unsigned best = 0;
+  if (row >= n) return;  // whole groups of 16; L >= 64: a whole wave or block
+  const T* src = scores + row * ld;
   Raw16 raw[R / V];
+  MaskVec<V, TAIL> ok[R / V];
 #pragma unroll
-  for (int i = 0; i < R / V; ++i)
-    raw[i] = RowVec<T, TAIL>::fetch(scores + row * ld, (i * L + lane) * V, K);
+  for (int i = 0; i < R / V; ++i) {
+    raw[i] = RowVec<T, TAIL>::fetch(src, (i * L + lane) * V, K);
+    if (MASKED) ok[i].fetch(mask, row, (i * L + lane) * V, K);
+  }
+  float v[R];
+  unsigned num[R], lost = 0;
+  bool nan = false;
 #pragma unroll
   for (int i = 0; i < R / V; ++i) {
     const int c = (i * L + lane) * V;
-    float v[V];
-    RowVec<T, TAIL>::value(raw[i], c, K, v);
+    float f[V];
+    RowVec<T, TAIL>::value(raw[i], c, K, f);
+    const unsigned in = MASKED ? ok[i].bits(mask, row, c, K) : 0u;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      key[i * V + j] = order_of(v[j], c + j < K && mask.at(row, c + j));
-      best = max(best, key[i * V + j]);
+      const bool there = MASKED ? (in >> j & 1) != 0 : c + (TAIL == TAIL_NONE ? 0 : j) < K;
+      v[i * V + j] = f[j];
+      // order_of() but for NaN, which is put right below where there is one
+      const unsigned b = __float_as_uint(f[j] + 0.f);
+      const unsigned key = b ^ ((unsigned)((int)b >> 31) | 0x80000000u);
+      nan |= there && f[j] != f[j];
+      if (sizeof(T) == 4) lost |= b & INDEX;
+      num[i * V + j] = there ? (key & ~INDEX) | (INDEX - (unsigned)(c + j)) : 0u;
     }
   }
-#pragma unroll
-  for (int o = L / 2; o > 0; o >>= 1) best = max(best, (unsigned)__shfl_xor((int)best, o, 64));
-  const float top = best ? score_of(best) : 0.f;
-  float total = 0.f;
-  if (!normalize) {
-#pragma unroll
-    for (int i = 0; i < R; ++i) total += key[i] ? expf(score_of(key[i]) - top) : 0.f;
-    total = lanes_sum<L>(total);
-  }
-  unsigned mine = 0;
-  int at = -1;
-  for (int j = 0; j < k; ++j) {
-    unsigned b = 0;
-    int bi = 0x7fffffff;
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-      const int c = ((i / V) * L + lane) * V + i % V;
-      if (key[i] > b) {
-        b = key[i];
-        bi = c;
-      }
-    }
-#pragma unroll
-    for (int o = L / 2; o > 0; o >>= 1) {
-      const unsigned ob = (unsigned)__shfl_xor((int)b, o, 64);
-      const int oi = __shfl_xor(bi, o, 64);
-      if (ob > b || (ob == b && oi < bi)) {
-        b = ob;
-        bi = oi;
-      }
-    }
+  if (__any(nan)) {
 #pragma unroll
     for (int i = 0; i < R; ++i)
-      if (((i / V) * L + lane) * V + i % V == bi) key[i] = 0;
-    if (lane == j && b) {
-      mine = b;
-      at = bi;
+      if (v[i] != v[i] && num[i]) num[i] |= ~INDEX;
+  }
+  if (sizeof(T) == 4) lost = group_all<L>(lost, Any(), s_all, turn);
+  unsigned limit = 0xffffffffu, before = 0, unsure = 0;
+  int at = -1;
+  bool left = true;
+  const int rounds = sizeof(T) == 4 ? k + 1 : k;
+  for (int j = 0; j < rounds; ++j) {
+    unsigned d = 0xffffffffu;
+#pragma unroll
+    for (int i = 0; i < R; ++i) d = min(d, limit - num[i]);
+    d = group_all<L>(d, Least(), s_all, turn);
+    const unsigned best = limit - d;
+    left = left && best > NONE;
+    if (sizeof(T) == 4) unsure |= j > 0 && left && ((best ^ before) & ~INDEX) == 0;
+    before = best;
+    limit = best - 1;
+    if (lane == j && j < k && left) at = (int)(INDEX - (best & INDEX));
+  }
+  if (sizeof(T) == 4) {
+    // the same for a row's threads; a wave of several rows does all of them again
+    const bool again = L > 64 ? (unsure && lost) : __any(unsure && lost);
+    if (again) {
+      unsigned key[R];
+#pragma unroll
+      for (int i = 0; i < R; ++i) key[i] = order_of(v[i], num[i] > NONE);
+      at = -1;
+      for (int j = 0; j < k; ++j) {
+        unsigned b = 0;
+        int bi = 0x7fffffff;
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+          if (key[i] > b) {
+            b = key[i];
+            bi = column<R>(i, V, L, lane);
+          }
+        }
+        const unsigned most = group_all<L>(b, Most(), s_all, turn);
+        bi = (int)group_all<L>(b == most ? (unsigned)bi : 0x7fffffffu, Least(), s_all, turn);
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+          if (column<R>(i, V, L, lane) == bi) key[i] = 0;
+        if (lane == j && most) at = bi;
+      }
     }
   }
-  const float e = mine ? expf(score_of(mine) - top) : 0.f;
-  if (normalize) total = lanes_sum<L>(e);
+  // the chosen are in lanes 0 .. k - 1 of the row
+  const float mine = at >= 0 ? up(src[at]) : 0.f;
+  float first = mine;
+  if constexpr (L > 64) {
+    unsigned* p = s_all[turn];
+    turn ^= 1;
+    if (threadIdx.x == 0) p[0] = __float_as_uint(mine);
+    __syncthreads();
+    first = __uint_as_float(p[0]);
+  } else {
+    first = __shfl(mine, (threadIdx.x & 63) / L * L, 64);
+  }
+  const float e = at >= 0 ? expf(mine - first) : 0.f;
+  float sum = normalize ? e : 0.f;
+  if (!normalize) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) sum += num[i] > NONE ? expf(v[i] - first) : 0.f;
+  }
+  sum = __uint_as_float(group_all<L>(__float_as_uint(sum), Sum(), s_all, turn));
   if (lane < k) {
-    w[row * k + lane] = mine ? e / total : 0.f;
+    w[row * k + lane] = at >= 0 ? e / sum : 0.f;
     labels[row * k + lane] = at;
   }
   if (stat && lane == 0) {
-    stat[2 * row] = top;
-    stat[2 * row + 1] = best ? 1.f / total : 0.f;
+    stat[2 * row] = first;
+    stat[2 * row + 1] = at >= 0 ? 1.f / sum : 0.f;
   }
 }
 
@@ -125,8 +251,7 @@ __device__ __forceinline__ void take_larger(unsigned& b, int& bi, unsigned ob, i
   }
 }
 
-// Any number of clusters: a block per row, which is read again in every round (from the
-// caches).  What is left is what comes after the last choice in the order.
+// More clusters: a block per row, which is read again in every round (from the caches).  What is left is what comes after the last choice in the order.
 template <typename T>
 __global__ __launch_bounds__(GATE_BLOCK) void gate_wide_kernel(
     const T* __restrict__ scores, int64_t ld, Mask mask, int64_t n, int K, int k, bool normalize,
@@ -192,39 +317,54 @@ __global__ __launch_bounds__(GATE_BLOCK) void gate_wide_kernel(
   }
 }
 
-// The gradient: L lanes per row write what every place gets and then, after those stores
-// have arrived, the chosen places.
+// The gradient: L lanes per row write what every place gets, U vectors at a time, and then,
+// after those stores have arrived, the chosen places.
 template <typename T, int L, int TAIL>
 __global__ __launch_bounds__(GATE_BLOCK) void gate_bwd_kernel(
     const T* __restrict__ scores, int64_t ld, Mask mask, const float* __restrict__ w,
     const int* __restrict__ labels, const float* __restrict__ stat, const float* __restrict__ dw,
     int64_t n, int K, int k, bool normalize, T* __restrict__ ds) {
-  constexpr int V = Vec<T>::N;
+  constexpr int V = Vec<T>::N, U = 2;
   const int lane = threadIdx.x % L;
   const int64_t row = (int64_t)blockIdx.x * (GATE_BLOCK / L) + threadIdx.x / L;
   if (row >= n) return;
   const float wj = lane < k ? w[row * k + lane] : 0.f;
   const float dj = lane < k ? dw[row * k + lane] : 0.f;
   const int at = lane < k ? labels[row * k + lane] : -1;
-  const float mean = lanes_sum<L>(at >= 0 ? wj * dj : 0.f);
   float top = 0.f, scale = 0.f;
   if (!normalize) {
     top = stat[2 * row];
-    scale = stat[2 * row + 1] * mean;
+    scale = stat[2 * row + 1];
   }
-  for (int c = lane * V; c < K; c += L * V) {
-    float v[V];
+  if (normalize) {  // while those loads are on their way
+    const float zero[V] = {};
+    for (int c = lane * V; c < K; c += L * V) RowVec<T, TAIL>::store(ds + row * K, c, K, zero);
+  }
+  const float mean = lanes_sum<L>(at >= 0 ? wj * dj : 0.f);
+  scale *= mean;
+  if (!normalize) {
+    for (int c0 = lane * V; c0 < K; c0 += L * V * U) {
+      float v[U][V];
+      Raw16 raw[U];
+      MaskVec<V, TAIL> ok[U];
 #pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = 0.f;
-    if (!normalize) {
-      RowVec<T, TAIL>::value(RowVec<T, TAIL>::fetch(scores + row * ld, c, K), c, K, v);
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const bool in = c + j < K && mask.at(row, c + j) && v[j] != -INFINITY;
-        v[j] = in ? -expf(v[j] - top) * scale : 0.f;
+      for (int u = 0; u < U; ++u) {
+        raw[u] = RowVec<T, TAIL>::fetch(scores + row * ld, c0 + u * L * V, K);
+        ok[u].fetch(mask, row, c0 + u * L * V, K);
       }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int c = c0 + u * L * V;
+        RowVec<T, TAIL>::value(raw[u], c, K, v[u]);
+        const unsigned in = ok[u].bits(mask, row, c, K);
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          v[u][j] = (in >> j & 1) && v[u][j] != -INFINITY ? -expf(v[u][j] - top) * scale : 0.f;
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (c0 + u * L * V < K) RowVec<T, TAIL>::store(ds + row * K, c0 + u * L * V, K, v[u]);
     }
-    RowVec<T, TAIL>::store(ds + row * K, c, K, v);
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   if (at >= 0 && at < K) ds[row * K + at] = down<T>(wj * (dj - mean));
@@ -250,14 +390,23 @@ int tdc_topk_gate(int dtype, const void* scores, int64_t ld, const uint8_t* mask
     };
     return with_tail(K, Vec<T>::N, [&](auto tail) {
       constexpr int TAIL = decltype(tail)::value;
-      if (K <= 128)
-        go(gate_kernel<T, 16, 8, TAIL>, 16);
-      else if (K <= 256)
-        go(gate_kernel<T, 16, 16, TAIL>, 16);
-      else if (K <= 1024)
-        go(gate_kernel<T, 64, 16, TAIL>, 64);
+      auto one = [&](auto masked) {
+        constexpr bool MASKED = decltype(masked)::value;
+        if (K <= 128)
+          go(gate_kernel<T, 16, 8, TAIL, MASKED>, 16);
+        else if (K <= 256)
+          go(gate_kernel<T, 16, 16, TAIL, MASKED>, 16);
+        else if (K <= 1024)
+          go(gate_kernel<T, 64, 16, TAIL, MASKED>, 64);
+        else if (K <= 4096)
+          go(gate_kernel<T, 256, 16, TAIL, MASKED>, 256);
+        else
+          go(gate_wide_kernel<T>, GATE_BLOCK);
+      };
+      if (mask)
+        one(std::true_type());
       else
-        go(gate_wide_kernel<T>, GATE_BLOCK);
+        one(std::false_type());
       TDC_CHECK_LAUNCH();
       return 0;
     });

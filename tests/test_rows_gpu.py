@@ -176,6 +176,24 @@ def test_gate(gpu, clusters, k, dtype):
             assert torch.equal(again[0], w) and torch.equal(again[1], lab)
 
 
+@pytest.mark.parametrize("clusters", [90, 256, 1000, 4096, 5000])
+def test_gate_scores_that_differ_in_their_last_bits(gpu, clusters):
+    g = torch.Generator().manual_seed(clusters)
+    step = 2.0 ** -23
+    rows = [1 + step * torch.randperm(clusters, generator=g).float(),
+            -1 - step * torch.randperm(clusters, generator=g).float(),
+            1 + step * (torch.randperm(clusters, generator=g) // 3).float(),   # ties among them
+            torch.randn(clusters, generator=g)]
+    rows[3][5] = rows[3].max() * (1 + 2 * step)                                # one close pair
+    s = torch.stack(rows)
+    for k in (1, 8, 16):
+        for normalize in (True, False):
+            w, lab = tdc.topk_gate(s.to(gpu), k, normalize=normalize)
+            ww, wl = rc.gate(s, k, None, normalize)
+            assert torch.equal(lab.cpu(), wl)
+            rc.close(w, ww, torch.float32, scale=torch.ones(1))
+
+
 def test_gate_nan_and_inf_that_are_allowed(gpu):
     for clusters in (3, 300, 2000):
         s = torch.zeros(2, clusters, device=gpu)
