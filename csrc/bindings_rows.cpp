@@ -114,7 +114,7 @@ std::vector<Tensor> norm_impl(const Tensor& x, const OptTensor& w, const OptTens
     res.push_back(rstd);
   }
   check(tdc_rms_norm(code, x.data_ptr(), x.stride(0), has(r) ? r->data_ptr() : nullptr,
-                     has(r) ? r->stride(0) : 0, wp, w32, n, (int)d, (float)eps,
+                     has(r) ? r->stride(0) : 0, wp, w32, n, (int)d, eps,
                      y.defined() ? y.data_ptr() : nullptr, q.defined() ? q.data_ptr() : nullptr,
                      s.defined() ? s.data_ptr() : nullptr, (int)fp8_width,
                      h.defined() ? h.data_ptr() : nullptr,

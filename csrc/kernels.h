@@ -241,7 +241,7 @@ int tdc_quant_fp8(int src_dtype, const void* X, int64_t rows, int64_t valid, int
 // RMS norm (rows_norm.hip): h = x + r in the rows' type (r nullable: h = x, not written), y or,
 // with q, e4m3 [n, dp] + E8M0 s [n, dp / 32] = h rstd w; rstd (nullable) fp32 [n]; d <= 16384.
 int tdc_rms_norm(int dtype, const void* x, int64_t ldx, const void* r, int64_t ldr, const void* w,
-                 int w32, int64_t n, int d, float eps, void* y, void* q, void* s, int dp, void* h,
+                 int w32, int64_t n, int d, double eps, void* y, void* q, void* s, int dp, void* h,
                  float* rstd, hipStream_t stream);
 // dx [n, d] (+ dh, nullable) and, with dw, dw [d] through part fp32 [parts, d] scratch.
 int tdc_rms_norm_bwd_parts(int64_t n, int cus);

@@ -91,12 +91,10 @@ template <typename T, int TAIL> struct RowVec {
       __builtin_memcpy(&r.w[0], &lo, 8);
       __builtin_memcpy(&r.w[2], &hi, 8);
       unpack<T>(r, v);
+    } else if constexpr (TAIL == TAIL_NONE) {
+      unpack<T>(if_kept(c < width, r), v);
     } else {
       unpack<T>(r, v);
-      if constexpr (TAIL == TAIL_NONE) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = c < width ? v[i] : 0.f;
-      }
     }
   }
   static __device__ __forceinline__ void store(T* __restrict__ row, int c, int width,
@@ -121,26 +119,52 @@ template <typename F> int with_tail(int d, int n, F&& f) {
   return f(std::integral_constant<int, TAIL_NONE>());
 }
 
-// Sum over G neighbouring lanes (a power of two up to 64), the same value in each.
-template <int G> __device__ __forceinline__ float lanes_sum(float v) {
-#pragma unroll
-  for (int o = G / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+// The lane of this 16-lane row that DPP control CTRL names.
+template <int CTRL> __device__ __forceinline__ unsigned dpp(unsigned v) {
+  return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
+}
+template <int CTRL> __device__ __forceinline__ float dpp(float v) {
+  return __uint_as_float(dpp<CTRL>(__float_as_uint(v)));
+}
+template <int CTRL> __device__ __forceinline__ double dpp(double v) {
+  return __hiloint2double((int)dpp<CTRL>((unsigned)__double2hiint(v)),
+                          (int)dpp<CTRL>((unsigned)__double2loint(v)));
+}
+constexpr int DPP_XOR1 = 0xb1, DPP_XOR2 = 0x4e;  // quad_perm [1,0,3,2] and [2,3,0,1]
+constexpr int DPP_HALF_MIRROR = 0x141;           // lane i of 8 from lane 7 - i
+constexpr int DPP_ROR = 0x120;                   // + n: rotate the row by n lanes
+
+// Sum over G neighbouring lanes (4 to 64, a power of two), the same value in each: rotations
+// and quad permutations within a row of 16, then across rows.
+template <int G, typename A> __device__ __forceinline__ A lanes_sum(A v) {
+  if constexpr (G >= 16) {
+    v += dpp<DPP_ROR + 8>(v);
+    v += dpp<DPP_ROR + 4>(v);
+    v += dpp<DPP_ROR + 2>(v);
+    v += dpp<DPP_ROR + 1>(v);
+    if constexpr (G >= 32) v += __shfl_xor(v, 16, 64);
+    if constexpr (G >= 64) v += __shfl_xor(v, 32, 64);
+  } else {
+    v += dpp<DPP_XOR1>(v);
+    v += dpp<DPP_XOR2>(v);
+    if constexpr (G >= 8) v += dpp<DPP_HALF_MIRROR>(v);
+  }
   return v;
 }
 
 // Sum over the G threads of a row: G <= 64 within the wave, above through LDS, where the
 // block is the row (G == blockDim.x).  `turn` alternates between two LDS rows, so one
 // barrier per sum is enough.
-template <int G> __device__ __forceinline__ float group_sum(float v, float (*s)[16], int& turn) {
+template <int G, typename A> __device__ __forceinline__ A group_sum(A v, A (*s)[16], int& turn) {
   if constexpr (G <= 64) {
     return lanes_sum<G>(v);
   } else {
     v = lanes_sum<64>(v);
-    float* p = s[turn];
+    A* p = s[turn];
     turn ^= 1;
     if ((threadIdx.x & 63) == 0) p[threadIdx.x >> 6] = v;
     __syncthreads();
-    float t = 0.f;
+    A t = 0;
 #pragma unroll
     for (int i = 0; i < G / 64; ++i) t += p[i];
     return t;

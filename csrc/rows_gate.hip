@@ -16,7 +16,7 @@
 // limit wraps around to more than the rest: 1.5 instructions per score and round, nothing
 // is taken out.  Where fp32 loses bits that are not zero and two neighbours among the first
 // k + 1 choices agree in the bits that are left, the rows of that wave are chosen again by
-// the whole scores.  65536 x 256 fp32, k = 8: @@ us, 37 with whole scores in every round.
+// the whole scores.  65536 x 256 fp32, k = 8: 21 us, 37 with whole scores in every round.
 #include "rows_common.h"
 
 namespace tdc {
@@ -77,14 +77,11 @@ template <int N, int TAIL> struct MaskVec {
 // Over the L threads of a row, the result in each: rotations within 16 lanes, the four rows
 // of a wave through scalars, the waves of a block through LDS (two rows in turn, one
 // barrier).
-template <int CTRL> __device__ __forceinline__ unsigned rotated(unsigned v) {
-  return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
-}
 template <typename Op> __device__ __forceinline__ unsigned row_all(unsigned v, Op op) {
-  v = op(v, rotated<0x128>(v));
-  v = op(v, rotated<0x124>(v));
-  v = op(v, rotated<0x122>(v));
-  return op(v, rotated<0x121>(v));
+  v = op(v, dpp<DPP_ROR + 8>(v));
+  v = op(v, dpp<DPP_ROR + 4>(v));
+  v = op(v, dpp<DPP_ROR + 2>(v));
+  return op(v, dpp<DPP_ROR + 1>(v));
 }
 template <int L, typename Op>
 __device__ __forceinline__ unsigned group_all(unsigned v, Op op, unsigned (*s)[4], int& turn) {
@@ -317,57 +314,65 @@ __global__ __launch_bounds__(GATE_BLOCK) void gate_wide_kernel(
   }
 }
 
-// The gradient: L lanes per row write what every place gets, U vectors at a time, and then,
-// after those stores have arrived, the chosen places.
+// The gradient: L lanes per row, U vectors of each at a time.  What the chosen places get on
+// top of the rest goes through LDS, so that every place is stored once (a second store of
+// the chosen places would have to wait until the first have arrived).  65536 x 256 fp32:
+// 17.6 us, bound by its 67 MB of stores and the latency of the few loads before them.
 template <typename T, int L, int TAIL>
 __global__ __launch_bounds__(GATE_BLOCK) void gate_bwd_kernel(
     const T* __restrict__ scores, int64_t ld, Mask mask, const float* __restrict__ w,
     const int* __restrict__ labels, const float* __restrict__ stat, const float* __restrict__ dw,
     int64_t n, int K, int k, bool normalize, T* __restrict__ ds) {
-  constexpr int V = Vec<T>::N, U = 2;
+  constexpr int V = Vec<T>::N, U = 16 / V;
+  constexpr int PASS = L * V * U;  // columns
+  __shared__ float more[GATE_BLOCK / L][PASS];
   const int lane = threadIdx.x % L;
+  float* mine = more[threadIdx.x / L];
   const int64_t row = (int64_t)blockIdx.x * (GATE_BLOCK / L) + threadIdx.x / L;
   if (row >= n) return;
   const float wj = lane < k ? w[row * k + lane] : 0.f;
   const float dj = lane < k ? dw[row * k + lane] : 0.f;
   const int at = lane < k ? labels[row * k + lane] : -1;
-  float top = 0.f, scale = 0.f;
-  if (!normalize) {
-    top = stat[2 * row];
-    scale = stat[2 * row + 1];
-  }
-  if (normalize) {  // while those loads are on their way
-    const float zero[V] = {};
-    for (int c = lane * V; c < K; c += L * V) RowVec<T, TAIL>::store(ds + row * K, c, K, zero);
-  }
+  const float top = normalize ? 0.f : stat[2 * row];
+  const float inv = normalize ? 0.f : stat[2 * row + 1];
   const float mean = lanes_sum<L>(at >= 0 ? wj * dj : 0.f);
-  scale *= mean;
-  if (!normalize) {
-    for (int c0 = lane * V; c0 < K; c0 += L * V * U) {
-      float v[U][V];
-      Raw16 raw[U];
-      MaskVec<V, TAIL> ok[U];
+  const float gain = wj * (normalize ? dj - mean : dj);
+  for (int c0 = 0; c0 < K; c0 += PASS) {
+    Raw16 raw[U];
+    MaskVec<V, TAIL> ok[U];
+    if (!normalize) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        raw[u] = RowVec<T, TAIL>::fetch(scores + row * ld, c0 + u * L * V, K);
-        ok[u].fetch(mask, row, c0 + u * L * V, K);
+        raw[u] = RowVec<T, TAIL>::fetch(scores + row * ld, c0 + (u * L + lane) * V, K);
+        ok[u].fetch(mask, row, c0 + (u * L + lane) * V, K);
       }
+    }
+    // a row's part of LDS is its own lanes': they run together, in the order of the program
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int c = c0 + u * L * V;
-        RowVec<T, TAIL>::value(raw[u], c, K, v[u]);
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < V; ++j) mine[(u * L + lane) * V + j] = 0.f;
+    __builtin_amdgcn_wave_barrier();
+    if (at >= c0 && at < c0 + PASS && at < K) mine[at - c0] = gain;
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int c = c0 + (u * L + lane) * V;
+      float v[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] = mine[(u * L + lane) * V + j];
+      if (!normalize) {
+        float f[V];
+        RowVec<T, TAIL>::value(raw[u], c, K, f);
         const unsigned in = ok[u].bits(mask, row, c, K);
 #pragma unroll
         for (int j = 0; j < V; ++j)
-          v[u][j] = (in >> j & 1) && v[u][j] != -INFINITY ? -expf(v[u][j] - top) * scale : 0.f;
+          if ((in >> j & 1) && f[j] != -INFINITY) v[j] -= expf(f[j] - top) * inv * mean;
       }
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (c0 + u * L * V < K) RowVec<T, TAIL>::store(ds + row * K, c0 + u * L * V, K, v[u]);
+      if (c < K) RowVec<T, TAIL>::store(ds + row * K, c, K, v);
     }
+    __builtin_amdgcn_wave_barrier();
   }
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  if (at >= 0 && at < K) ds[row * K + at] = down<T>(wj * (dj - mean));
 }
 
 }  // namespace rows

@@ -10,7 +10,7 @@
 //   fp8: per 32 columns e = floor(log2 max|y|) - 7, q = e4m3(y 2^-e) (the layout of
 //        quant_fp8_kernel), columns past the row's end are zero
 //
-// All sums are fp32; y, h and dx are rounded once.  Bound by memory: the row lives in
+// The sums are fp32 (fp64 for fp8 rows); y, h, dx and q are rounded once.  Bound by memory: the row lives in
 // registers between its one read and its one write.  A row is spread over G threads with
 // NV vectors of 16 bytes each; several rows share a wave when they are short, a block
 // works on one row when it is long.
@@ -57,41 +57,54 @@ template <typename T, int TAIL> struct WeightVec {
 };
 
 // N values of one lane to e4m3 with the exponent of their block of 32 columns (32 / N
-// neighbouring lanes).  The block's largest value lies in [2^7, 2^8) after the scaling:
-// no saturation.
+// neighbouring lanes).  The block's largest value lies in [2^7, 2^8) after the scaling: no
+// saturation.  The scale byte e + 127 is 7 less than the largest value's exponent field.
 template <int N>
 __device__ __forceinline__ void store_fp8(uint8_t* __restrict__ q, uint8_t* __restrict__ s, int c,
-                                          const float (&y)[N]) {
+                                          bool in, const float (&y)[N]) {
   float am = 0.f;
 #pragma unroll
   for (int i = 0; i < N; ++i) am = fmaxf(am, fabsf(y[i]));
-#pragma unroll
-  for (int o = 1; o < 32 / N; o <<= 1) am = fmaxf(am, __shfl_xor(am, o, 64));
-  int e = am > 0.f ? ilogbf(am) - 7 : -127;
-  e = e < -127 ? -127 : (e > 126 ? 126 : e);
-  const float inv = ldexpf(1.f, -e);
+  am = fmaxf(am, dpp<DPP_XOR1>(am));
+  am = fmaxf(am, dpp<DPP_XOR2>(am));
+  if constexpr (N == 4) am = fmaxf(am, dpp<DPP_HALF_MIRROR>(am));
+  const int byte = max((int)(__float_as_uint(am) >> 23) - 7, 0);
+  const float inv = __uint_as_float((unsigned)(254 - byte) << 23);
   int p[N / 4];
 #pragma unroll
   for (int i = 0; i < N / 4; ++i) {
     p[i] = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * i] * inv, y[4 * i + 1] * inv, 0, false);
     p[i] = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * i + 2] * inv, y[4 * i + 3] * inv, p[i], true);
   }
+  if (!in) return;
   if constexpr (N == 8)
     *reinterpret_cast<int2*>(q + c) = make_int2(p[0], p[1]);
   else
     *reinterpret_cast<int*>(q + c) = p[0];
-  if (c % 32 == 0) s[c / 32] = (uint8_t)(e + 127);
+  if (c % 32 == 0) s[c / 32] = (uint8_t)byte;
 }
 
+// x as a float of 21 bits whose last one also stands for all that follow it: rounding it
+// further, to e4m3, gives what rounding x does, and its exponent is x's.
+__device__ __forceinline__ float sticky_float(double x) {
+  const unsigned rest = min((unsigned)__double2loint(x), 1u);
+  return (float)__hiloint2double(__double2hiint(x) | (int)rest, 0);
+}
+
+// FP8: the row's sum and products are fp64.  A value next to the border of two e4m3 values
+// lands a step of 1/8 away when fp32 puts it on the other side, about one in a million; in
+// fp64 q is the rounding of the norm itself, whatever the order of the sum.  It
+// stays bound by memory: 262144 x 768 bf16 in 258 us, 5.5 TB/s.
 template <typename T, int G, int NV, int TAIL, bool FP8>
 __global__ __launch_bounds__(block_of<G>()) void norm_kernel(
     const T* __restrict__ x, int64_t ldx, const T* __restrict__ r, int64_t ldr,
-    const void* __restrict__ w, bool w32, int64_t n, int d, float eps, T* __restrict__ y,
+    const void* __restrict__ w, bool w32, int64_t n, int d, double eps, T* __restrict__ y,
     uint8_t* __restrict__ q, uint8_t* __restrict__ s, int dp, T* __restrict__ h,
     float* __restrict__ rstd) {
   constexpr int N = Vec<T>::N;
   using R = RowVec<T, TAIL>;
-  __shared__ float part[2][16];
+  using A = std::conditional_t<FP8, double, float>;
+  __shared__ A part[2][16];
   int turn = 0;
   const int lane = threadIdx.x % G;
   const int64_t row = (int64_t)blockIdx.x * (block_of<G>() / G) + threadIdx.x / G;
@@ -107,7 +120,7 @@ __global__ __launch_bounds__(block_of<G>()) void norm_kernel(
 #pragma unroll
   for (int i = 0; i < NV; ++i) wr[i].fetch(w, w32, (i * G + lane) * N, d);
   float v[NV][N];
-  float sq = 0.f;
+  A sq = 0;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c = (i * G + lane) * N;
@@ -120,24 +133,29 @@ __global__ __launch_bounds__(block_of<G>()) void norm_kernel(
       R::store(h + row * d, c, d, v[i]);
     }
 #pragma unroll
-    for (int j = 0; j < N; ++j) sq = fmaf(v[i][j], v[i][j], sq);
+    for (int j = 0; j < N; ++j) sq = std::fma((A)v[i][j], (A)v[i][j], sq);
   }
   sq = group_sum<G>(sq, part, turn);
-  const float rs = 1.f / sqrtf(sq / (float)d + eps);
-  if (rstd && lane == 0) rstd[row] = rs;
+  const A rs = (A)1 / std::sqrt(sq / (A)d + (A)eps);
+  if (rstd && lane == 0) rstd[row] = (float)rs;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c = (i * G + lane) * N;
     float t[N];
     wr[i].value(w, w32, c, d, t);
-#pragma unroll
-    for (int j = 0; j < N; ++j) t[j] = v[i][j] * rs * t[j];
     if constexpr (FP8) {
       // the exponent's lanes all take part; a block of 32 is stored or not as a whole
 #pragma unroll
-      for (int j = 0; j < N; ++j) t[j] = c + j < d ? t[j] : 0.f;
-      if (c < dp) store_fp8<N>(q + row * dp, s + row * (dp / 32), c, t);
+      for (int j = 0; j < N; ++j) {
+        const float f = sticky_float((double)v[i][j] * (double)t[j] * rs);
+        // a mask, not a choice: that would be a branch around the fp64 products
+        const int in = TAIL == TAIL_NONE ? c - d : c + j - d;
+        t[j] = __uint_as_float(__float_as_uint(f) & (unsigned)(in >> 31));
+      }
+      store_fp8<N>(q + row * dp, s + row * (dp / 32), c, c < dp, t);
     } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j) t[j] = v[i][j] * rs * t[j];
       R::store(y + row * d, c, d, t);
     }
   }
@@ -265,46 +283,56 @@ __global__ __launch_bounds__(1024) void dw_kernel(const float* __restrict__ part
   }
 }
 
-// q 2^e, one 16-byte vector of the result per thread, a row per grid row block: the reads
-// and writes of a wave are contiguous.  2^e is built from its bits (scale 0 is the subnormal
-// 2^-127), the product is exact.
-template <typename T, int TAIL>
-__global__ __launch_bounds__(BLOCK) void dequant_kernel(const uint8_t* __restrict__ q,
-                                                        const uint8_t* __restrict__ s, int64_t n,
-                                                        int d, int dp, T* __restrict__ out,
-                                                        int rows) {
+// q 2^e: a row is spread over G threads as in the norm, all loads first.  2^e is built from
+// its bits (scale 0 is the subnormal 2^-127), the product is exact.
+template <typename T, int G, int NV, int TAIL>
+__global__ __launch_bounds__(block_of<G>()) void dequant_kernel(const uint8_t* __restrict__ q,
+                                                                const uint8_t* __restrict__ s,
+                                                                int64_t n, int d, int dp,
+                                                                T* __restrict__ out) {
   constexpr int N = Vec<T>::N;
-  const int per = BLOCK / rows;  // threads of a row
-  const int64_t row = (int64_t)blockIdx.x * rows + threadIdx.x / per;
+  const int lane = threadIdx.x % G;
+  const int64_t row = (int64_t)blockIdx.x * (block_of<G>() / G) + threadIdx.x / G;
   if (row >= n) return;
-  for (int c = (threadIdx.x % per) * N; c < d; c += per * N) {
-    unsigned p[N / 4];
-    __builtin_memcpy(p, q + row * dp + c, N);
-    const unsigned e = s[row * (dp / 32) + c / 32];
-    const float f = __uint_as_float(e ? e << 23 : 0x00400000u);
+  unsigned p[NV][N / 4], e[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = min((i * G + lane) * N, dp - N);
+    __builtin_memcpy(p[i], __builtin_assume_aligned(q + row * dp + c, N), N);
+    e[i] = s[row * (dp / 32) + c / 32];
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const float f = __uint_as_float(e[i] ? e[i] << 23 : 0x00400000u);
     float v[N];
 #pragma unroll
     for (int k = 0; k < N / 4; ++k) {
-      v[4 * k] = __builtin_amdgcn_cvt_f32_fp8((int)p[k], 0) * f;
-      v[4 * k + 1] = __builtin_amdgcn_cvt_f32_fp8((int)p[k], 1) * f;
-      v[4 * k + 2] = __builtin_amdgcn_cvt_f32_fp8((int)p[k], 2) * f;
-      v[4 * k + 3] = __builtin_amdgcn_cvt_f32_fp8((int)p[k], 3) * f;
+      v[4 * k] = __builtin_amdgcn_cvt_f32_fp8((int)p[i][k], 0) * f;
+      v[4 * k + 1] = __builtin_amdgcn_cvt_f32_fp8((int)p[i][k], 1) * f;
+      v[4 * k + 2] = __builtin_amdgcn_cvt_f32_fp8((int)p[i][k], 2) * f;
+      v[4 * k + 3] = __builtin_amdgcn_cvt_f32_fp8((int)p[i][k], 3) * f;
     }
-    RowVec<T, TAIL>::store(out + row * d, c, d, v);
+    const int c = (i * G + lane) * N;
+    if (c < d) RowVec<T, TAIL>::store(out + row * d, c, d, v);
   }
 }
 
-// Calls f(G, NV) for a row of `width` in vectors of N elements (16 bytes): the fewest threads that hold it
-// in at most 4 vectors each, a wave from 17 vectors on, so that the row's sum needs no
-// barrier up to 256 vectors (4 KiB).
+// Calls f(G, NV) for a row of `width` in vectors of N elements (16 bytes): threads and
+// vectors of each that hold the row with few to spare (768 bf16: 32 x 3; as 64 x 2 with a
+// quarter idle the fp8 norm took 20 % longer), within a wave, where the row's sum needs no
+// barrier, up to 256 vectors (4 KiB).
 template <int N, typename F> int with_shape(int width, F&& f) {
   const int vecs = (width + N - 1) / N;
 #define TDC_SHAPE(G, NV) f(std::integral_constant<int, G>(), std::integral_constant<int, NV>())
   if (vecs <= 16) return TDC_SHAPE(16, 1);
+  if (vecs <= 32) return TDC_SHAPE(32, 1);
   if (vecs <= 64) return TDC_SHAPE(64, 1);
+  if (vecs <= 96) return TDC_SHAPE(32, 3);
   if (vecs <= 128) return TDC_SHAPE(64, 2);
+  if (vecs <= 192) return TDC_SHAPE(64, 3);
   if (vecs <= 256) return TDC_SHAPE(64, 4);
   if (vecs <= 512) return TDC_SHAPE(256, 2);
+  if (vecs <= 768) return TDC_SHAPE(256, 3);
   if (vecs <= 1024) return TDC_SHAPE(256, 4);
   if (vecs <= 2048) return TDC_SHAPE(1024, 2);
   if constexpr (N == 4)  // 16384 columns of fp32
@@ -319,7 +347,7 @@ template <int N, typename F> int with_shape(int width, F&& f) {
 using namespace tdc::rows;
 
 int tdc_rms_norm(int dtype, const void* x, int64_t ldx, const void* r, int64_t ldr, const void* w,
-                 int w32, int64_t n, int d, float eps, void* y, void* q, void* s, int dp, void* h,
+                 int w32, int64_t n, int d, double eps, void* y, void* q, void* s, int dp, void* h,
                  float* rstd, hipStream_t stream) {
   if (n == 0) return 0;
   return with_type(dtype, [&](auto t) {
@@ -339,7 +367,7 @@ int tdc_rms_norm(int dtype, const void* x, int64_t ldx, const void* r, int64_t l
         constexpr int TAIL = decltype(tail)::value;
         // an fp8 row has 256 columns or more, and a row shorter than a vector few threads
         if (q) {
-          if constexpr (G > 16 && (TAIL != TAIL_SHORT || (G == 64 && NV == 1)))
+          if constexpr (G > 16 && (TAIL != TAIL_SHORT || (G <= 64 && NV == 1)))
             go(norm_kernel<T, G, NV, TAIL, true>);
           else
             return (int)hipErrorInvalidValue;
@@ -406,18 +434,19 @@ int tdc_dequant_fp8(int dtype, const void* q, const void* s, int64_t n, int d, i
   if (dp % 32 != 0 || d > dp) return (int)hipErrorInvalidValue;
   return with_type(dtype, [&](auto t) {
     using T = decltype(t);
-    // rows of a block: as many as its threads cover once
-    const int vecs = (d + Vec<T>::N - 1) / Vec<T>::N;
-    int rows = 1;
-    while (rows < 32 && rows * 2 * vecs <= BLOCK) rows *= 2;
-    const int64_t blocks = (n + rows - 1) / rows;
-    if (blocks > 0x7fffffff) return (int)hipErrorInvalidValue;
-    return with_tail(d, Vec<T>::N, [&](auto tail) {
-      constexpr int TAIL = decltype(tail)::value;
-      hipLaunchKernelGGL((dequant_kernel<T, TAIL>), dim3((unsigned)blocks), dim3(BLOCK), 0, stream,
-                         (const uint8_t*)q, (const uint8_t*)s, n, d, dp, (T*)out, rows);
-      TDC_CHECK_LAUNCH();
-      return 0;
+    return with_shape<Vec<T>::N>(d, [&](auto g, auto nv) {
+      constexpr int G = decltype(g)::value, NV = decltype(nv)::value;
+      constexpr int B = block_of<G>();
+      const int64_t blocks = (n + B / G - 1) / (B / G);
+      if (blocks > 0x7fffffff) return (int)hipErrorInvalidValue;
+      return with_tail(d, Vec<T>::N, [&](auto tail) {
+        constexpr int TAIL = decltype(tail)::value;
+        if constexpr (TAIL != TAIL_SHORT || G == 16)
+          hipLaunchKernelGGL((dequant_kernel<T, G, NV, TAIL>), dim3((unsigned)blocks), dim3(B), 0,
+                             stream, (const uint8_t*)q, (const uint8_t*)s, n, d, dp, (T*)out);
+        TDC_CHECK_LAUNCH();
+        return 0;
+      });
     });
   });
 }

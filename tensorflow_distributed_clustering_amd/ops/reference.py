@@ -176,31 +176,35 @@ def kmeanspp(x: torch.Tensor, k: int, generator: torch.Generator,
 
 
 # ----------------------------------------------------------------- row operators
-# The formulas of ops/rows.py in fp32 (differentiable by autograd): the CPU path.
+# The formulas of ops/rows.py in fp32 (fp64 for fp8 rows), differentiable by autograd: the
+# CPU path.
 
 def rms_norm(x, weight, residual, eps: float):
     h = x if residual is None else (x.float() + residual.float()).to(x.dtype)
-    y = _normed(h, weight, eps).to(x.dtype)
+    y = _normed(h, weight, eps, torch.float32).to(x.dtype)
     return y if residual is None else (y, h)
 
 
-def _normed(h, weight, eps: float):
-    hf = h.float()
+def _normed(h, weight, eps: float, dtype):
+    hf = h.to(dtype)
     y = hf / torch.sqrt(hf.square().mean(1, keepdim=True) + eps)
-    return y if weight is None else y * weight.float()
+    return y if weight is None else y * weight.to(dtype)
 
 
 def rms_norm_fp8(x, weight, residual, eps: float, width: int):
     """(q e4m3 [N, width], scales uint8 [N, width / 32][, h]): exponent floor(log2 max) - 7
     per 32 columns, as the GPU quantiser."""
     h = x if residual is None else (x.float() + residual.float()).to(x.dtype)
-    y = torch.nn.functional.pad(_normed(h, weight, eps), (0, width - x.shape[1]))
+    # in fp64, so that q is the rounding of the norm itself
+    y = torch.nn.functional.pad(_normed(h, weight, eps, torch.float64), (0, width - x.shape[1]))
     b = y.view(y.shape[0], width // 32, 32)
     top = b.abs().nan_to_num(nan=0.0, posinf=math.inf).amax(2, keepdim=True)
     e = torch.frexp(top)[1] - 8
     e = torch.where(top > 0, e, -127)
-    e = torch.where(top.isinf(), 126, e).clamp(-127, 126)
-    q = torch.ldexp(b, -e).to(torch.float8_e4m3fn).view(y.shape)
+    e = torch.where(top.isinf(), 121, e).clamp(min=-127)
+    v = torch.ldexp(b, -e)
+    step = torch.ldexp(torch.ones_like(v), torch.frexp(v)[1].clamp(min=-5) - 4)
+    q = (torch.round(v / step) * step).to(torch.float8_e4m3fn).view(y.shape)
     out = (q, (e + 127).to(torch.uint8).squeeze(2))
     return out if residual is None else (*out, h)
 

@@ -133,8 +133,8 @@ def fp8_width(d: int) -> int:
 
 def rms_norm_fp8(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
                  residual: Optional[torch.Tensor] = None, eps: float = 1e-6):
-    """:func:`rms_norm` whose ``y`` is rounded from fp32 straight to :class:`Fp8Rows`, one
-    exponent per 32 columns.  Returns the rows, or ``(rows, h)`` with a residual.  For
+    """:func:`rms_norm` whose ``y`` is computed in fp64 and rounded once to
+    :class:`Fp8Rows`, one exponent per 32 columns.  Returns the rows, or ``(rows, h)`` with a residual.  For
     serving: it has no gradient, and refuses inputs that ask for one."""
     _check_norm(x, weight, residual, eps)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):

@@ -55,8 +55,7 @@ def norm_grads(h, weight, eps, dy, dh):
 
 
 def fp8(y64, width):
-    """(values, exponents) of rows in 64 bits as e4m3 with one exponent per 32 columns, and
-    half the distance of e4m3 values around each (what a rounding may move)."""
+    """(values, exponents) of rows in 64 bits as e4m3 with one exponent per 32 columns."""
     # on the CPU, where powers of two come out exact
     b = torch.nn.functional.pad(y64.cpu(), (0, width - y64.shape[1])).view(y64.shape[0], width // 32, 32)
     top = b.abs().amax(2, keepdim=True)
@@ -65,9 +64,7 @@ def fp8(y64, width):
     x = torch.where(v == 0, -6, torch.frexp(v)[1] - 1).clamp(min=-6)
     step = torch.ldexp(torch.ones_like(v), x - 3)
     q = torch.round(v / step) * step
-    flat = (y64.shape[0], width)
-    return (torch.ldexp(q, e).view(flat).to(y64.device), e.squeeze(2).to(y64.device),
-            torch.ldexp(step, e).view(flat).to(y64.device))
+    return torch.ldexp(q, e).view(y64.shape[0], width).to(y64.device), e.squeeze(2).to(y64.device)
 
 
 def gate(scores, k, mask, normalize, dw=None):

@@ -62,12 +62,9 @@ def test_norm_fp8(d):
     x[2] = 0
     rows = tdc.rms_norm_fp8(x, eps=1e-6)
     assert rows.shape == (5, d) and rows.q.shape[1] == R.fp8_width(d) and rows.q.shape[1] % 32 == 0
-    want, e, step = rc.fp8(rc.norm(x, None, 1e-6)[1], rows.q.shape[1])
+    want, e = rc.fp8(rc.norm(x, None, 1e-6)[1], rows.q.shape[1])
     assert torch.equal(rows.scales.int() - 127, e.int())
-    got = rows.dequantize(torch.bfloat16).double()
-    # a value within fp32 error of a border may round to the other side: one step
-    assert bool(((got - want[:, :d]).abs() <= step[:, :d] * 1.001).all())
-    assert float((got != want[:, :d]).double().mean()) < 1e-3
+    assert torch.equal(rows.dequantize(torch.bfloat16).double(), want[:, :d])
     assert bool((rows.q.float()[:, d:] == 0).all())
 
 

@@ -94,14 +94,11 @@ def test_norm_fp8(gpu, n, d, dtype):
     assert torch.equal(h.isnan(), x.isnan()) and torch.equal(h.nan_to_num(), rc.sum_kept(x, r).nan_to_num())
     assert rows.shape == (n, d)
     good = ~x.isnan().any(1)
-    want, e, step = rc.fp8(rc.norm(h[good], w, 1e-6)[1], rows.q.shape[1])
+    want, e = rc.fp8(rc.norm(h[good], w, 1e-6)[1], rows.q.shape[1])
     got = rows.dequantize(torch.float32)
     assert torch.equal(got[good], rows.dequantize(torch.bfloat16)[good].float())
     assert bool(got[~good].isnan().all())
-    far = (got[good].double() - want[:, :d]).abs()
-    assert bool((far <= step[:, :d] * 1.001).all())            # a border value rounds either way
-    assert float((far > 0).double().sum()) <= 1 + 1e-4 * far.numel()
-    assert float((rows.scales[good].int() - 127 != e).double().sum()) <= 1e-4 * e.numel()
+    assert torch.equal(got[good].double(), want[:, :d]) and torch.equal(rows.scales[good].int() - 127, e.int())
     assert not bool(rows.q.float()[good][:, d:].any())
 
 
