@@ -26,7 +26,8 @@ def strided(t, start=3, more=5):
 
 # ----------------------------------------------------------------- norm
 @pytest.mark.parametrize("n,d", [(1, 1), (5, 7), (17, 128), (3, 129), (1, 1024), (33, 768), (7, 1001),
-                                 (2100, 96), (600, 2048), (4, 4100), (5, 8200), (2, 16384), (0, 64)])
+                                 (2100, 96), (600, 2048), (4, 4100), (5, 8200), (2, 16384), (0, 64),
+                                 (9, 250), (3, 1300), (3, 5003), (2, 12001)])
 @pytest.mark.parametrize("dtype", rc.DTYPES)
 def test_norm_and_gradient(gpu, n, d, dtype):
     x, r = normal(gpu, 1, n, d, dtype=dtype), normal(gpu, 2, n, d, dtype=dtype, scale=3.0)
@@ -271,6 +272,60 @@ def test_group_and_combine(gpu, n, k, d, dtype):
             assert not bool(grads[1][~kept].any())
             only, = torch.autograd.grad(tdc.combine_rows(y, groups, wv), wv, dout)
             assert torch.equal(only, grads[1])
+
+
+# ----------------------------------------------------------------- large, streams
+def test_offsets_past_32_bits(gpu):
+    n, d = 140_000, 16384                            # 2.29e9 elements
+    x = torch.ones(n, d, dtype=torch.bfloat16, device=gpu)
+    x[-1] = normal(gpu, 1, d, dtype=torch.bfloat16)
+    y, h = tdc.rms_norm(x, residual=x[:1].expand(n, d))
+    want = rc.sum_kept(x[-1:], x[:1])
+    assert torch.equal(h[-1:], want) and bool((h[:2] == 2).all()) and bool((y[-2] == y[0]).all())
+    rc.close(y[-1:], rc.norm(want, None, 1e-6)[1], torch.bfloat16)
+    del y, h
+    rows = tdc.rms_norm_fp8(x)
+    assert torch.equal(tdc.Fp8Rows(rows.q[-1:], rows.scales[-1:], d).dequantize(torch.bfloat16),
+                       rows.dequantize(torch.bfloat16)[-1:])
+    del rows
+    groups = tdc.group_plan(torch.arange(n, device=gpu).flip(0).remainder(3), 3)
+    xg = tdc.group_rows(x, groups)
+    at = int(groups.pos[-1])
+    assert torch.equal(xg[at], x[-1]) and torch.equal(xg[-1], x[int(groups.order[-1])])
+    back = tdc.combine_rows(xg, groups)
+    assert torch.equal(back[-1], x[-1]) and torch.equal(back[0], x[0])
+    del xg, back, x
+    s = torch.zeros(600_000, 4096, dtype=torch.bfloat16, device=gpu)
+    s[-1, 4000], s[-1, 7] = 2.0, 1.0
+    s.requires_grad_()
+    w, lab = tdc.topk_gate(s, 2, normalize=False)
+    assert lab[-1].tolist() == [4000, 7] and lab[0].tolist() == [0, 1]
+    ds, = torch.autograd.grad(w, s, torch.tensor([1.0, 0.0], device=gpu).expand(600_000, 2))
+    _, _, want = rc.gate(s[-1:].detach().cpu(), 2, None, False, torch.tensor([[1.0, 0.0]]))
+    rc.close(ds[-1:], want, torch.bfloat16, scale=torch.ones(1))
+
+
+def test_two_streams_at_once_and_inference_mode(gpu):
+    x, w = normal(gpu, 1, 5000, 300, dtype=torch.bfloat16), normal(gpu, 2, 300)
+    s = normal(gpu, 3, 5000, 40)
+
+    def step(i):
+        y = tdc.rms_norm(x[i:], w)
+        wt, lab = tdc.topk_gate(s[i:], 3)
+        g = tdc.group_plan(lab, 40)
+        return tdc.combine_rows(tdc.group_rows(y, g), g, wt)
+
+    want = [step(i) for i in range(4)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    with torch.inference_mode():
+        for _ in range(5):
+            got = []
+            for i, st in enumerate(streams):
+                with torch.cuda.stream(st):
+                    got.append(step(i))
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
 # ----------------------------------------------------------------- together
