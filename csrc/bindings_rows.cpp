@@ -11,6 +11,8 @@
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 
+#include <algorithm>
+#include <cmath>
 #include <limits>
 
 #include "kernels.h"
@@ -31,7 +33,7 @@ int code_of(at::ScalarType t, const char* what) {
     case at::kFloat: return TDC_F32;
     case at::kHalf: return TDC_F16;
     case at::kBFloat16: return TDC_BF16;
-    default: TORCH_CHECK(false, "tdc: ", what, " must be fp32, fp16 or bf16, got ", t);
+    default: TORCH_CHECK_VALUE(false, what, " must be fp32, fp16 or bf16, got ", t);
   }
   return -1;
 }
@@ -43,34 +45,41 @@ void check(int err, const char* what) {
 
 bool has(const OptTensor& t) { return t.has_value() && t->defined(); }
 
-// Rows on the GPU with neighbouring columns.
+// Arguments that a caller gets wrong raise ValueError, as the checks of the CPU path do.
 void check_rows(const Tensor& x, const char* name) {
-  TORCH_CHECK(x.is_cuda() && x.dim() == 2 && (x.stride(1) == 1 || x.size(1) <= 1), "tdc: ", name,
-              " must be rows [N, D] on the GPU with contiguous columns");
+  TORCH_CHECK_VALUE(x.dim() == 2, name, " must be rows [N, D], got ", x.sizes());
+  TORCH_CHECK_VALUE(x.size(1) >= 1, name, " has no columns");
+  TORCH_CHECK_VALUE(x.stride(1) == 1 || x.size(1) == 1, name,
+                    " must have contiguous columns, got strides ", x.strides());
 }
 
 void check_like(const Tensor& t, const Tensor& x, const char* name) {
   check_rows(t, name);
-  TORCH_CHECK(t.device() == x.device() && t.scalar_type() == x.scalar_type() && t.sizes() == x.sizes(),
-              "tdc: ", name, " must have the shape, type and device of the rows");
+  TORCH_CHECK_VALUE(t.device() == x.device() && t.scalar_type() == x.scalar_type() &&
+                        t.sizes() == x.sizes(),
+                    name, " must have the shape, type and device of the rows");
 }
 
-// Weights of `n` elements: null, fp32 (w32) or the rows' type.
-const void* weights_of(const OptTensor& w, const Tensor& x, int64_t n, bool& w32) {
+// Weights of shape `sizes`: null, fp32 (w32) or the rows' type.
+const void* weights_of(const OptTensor& w, const Tensor& x, at::IntArrayRef sizes, const char* name,
+                       bool& w32) {
   w32 = true;
   if (!has(w)) return nullptr;
-  TORCH_CHECK(w->device() == x.device() && w->is_contiguous() && w->numel() == n,
-              "tdc: weights must be contiguous, on the rows' device and match their shape");
+  TORCH_CHECK_VALUE(w->sizes() == sizes && w->is_contiguous(), name, " must be contiguous ", sizes,
+                    ", got ", w->sizes());
+  TORCH_CHECK_VALUE(w->device() == x.device(), name, " is on ", w->device(), ", the rows on ",
+                    x.device());
   w32 = w->scalar_type() == at::kFloat;
-  TORCH_CHECK(w32 || w->scalar_type() == x.scalar_type(),
-              "tdc: weights must be fp32 or of the rows' type");
+  TORCH_CHECK_VALUE(w32 || w->scalar_type() == x.scalar_type(), name,
+                    " must be fp32 or of the rows' type, got ", w->scalar_type());
   return w->data_ptr();
 }
 
 void check_index(const Tensor& t, const Tensor& x, int64_t n, const char* name) {
-  TORCH_CHECK(t.device() == x.device() && t.scalar_type() == at::kInt && t.is_contiguous() &&
-                  t.numel() == n,
-              "tdc: ", name, " must be int32 [", n, "] on the rows' device");
+  TORCH_CHECK_VALUE(t.device() == x.device(), "the plan is on ", t.device(), ", the rows on ",
+                    x.device());
+  TORCH_CHECK_VALUE(t.scalar_type() == at::kInt && t.is_contiguous() && t.numel() == n, "tdc: ", name,
+                    " must be int32 [", n, "]");
 }
 
 int num_cus(const Tensor& t) {
@@ -87,12 +96,13 @@ std::vector<Tensor> norm_impl(const Tensor& x, const OptTensor& w, const OptTens
   check_rows(x, "x");
   const int64_t n = x.size(0), d = x.size(1);
   const int code = code_of(x.scalar_type(), "x");
-  TORCH_CHECK(d >= 1 && d <= MAX_WIDTH && fp8_width <= MAX_WIDTH, "tdc.rms_norm: 1 to ", MAX_WIDTH,
-              " columns, got ", d);
+  TORCH_CHECK_VALUE(d <= MAX_WIDTH && fp8_width <= MAX_WIDTH, "rms_norm takes up to ", MAX_WIDTH,
+                    " columns, got ", d);
+  TORCH_CHECK_VALUE(eps >= 0 && std::isfinite(eps), "eps must be finite and not negative, got ", eps);
   TORCH_CHECK(fp8_width == 0 || (fp8_width % 32 == 0 && fp8_width >= d), "tdc.rms_norm: fp8 width");
   if (has(r)) check_like(*r, x, "residual");
   bool w32;
-  const void* wp = weights_of(w, x, d, w32);
+  const void* wp = weights_of(w, x, {d}, "weight", w32);
   const DevGuard guard(x.device());
   std::vector<Tensor> res;
   Tensor q, s, y;
@@ -135,7 +145,7 @@ std::vector<Tensor> norm_bwd_impl(const Tensor& h, const OptTensor& w, const Ten
                   rstd.is_contiguous() && rstd.numel() == n, "tdc.rms_norm_bwd: rstd fp32 [N]");
   TORCH_CHECK(!want_dw || has(w), "tdc.rms_norm_bwd: dw needs the weights");
   bool w32;
-  const void* wp = weights_of(w, h, d, w32);
+  const void* wp = weights_of(w, h, {d}, "weight", w32);
   const DevGuard guard(h.device());
   Tensor dx = at::empty({n, d}, h.options());
   std::vector<Tensor> res = {dx};
@@ -180,9 +190,11 @@ struct MaskArg {
 MaskArg mask_of(const OptTensor& mask, const Tensor& like, int64_t n, int64_t K) {
   MaskArg m;
   if (!has(mask)) return m;
-  TORCH_CHECK(mask->device() == like.device() && mask->scalar_type() == at::kBool &&
-                  mask->dim() == 2 && mask->size(0) == n && mask->size(1) == K,
-              "tdc.topk_gate: mask must be bool [N, K] on the scores' device");
+  TORCH_CHECK_VALUE(mask->scalar_type() == at::kBool, "mask must be a bool tensor");
+  TORCH_CHECK_VALUE(mask->device() == like.device(), "mask is on ", mask->device(),
+                    ", the scores on ", like.device());
+  TORCH_CHECK_VALUE(mask->dim() == 2 && mask->size(0) == n && mask->size(1) == K,
+                    "mask must be [N, K], got ", mask->sizes());
   m.p = static_cast<const uint8_t*>(mask->data_ptr());
   m.rs = mask->stride(0);
   m.cs = mask->stride(1);
@@ -194,8 +206,9 @@ std::vector<Tensor> gate_impl(const Tensor& scores, const OptTensor& mask, int64
   check_rows(scores, "scores");
   const int64_t n = scores.size(0), K = scores.size(1);
   const int code = code_of(scores.scalar_type(), "scores");
-  TORCH_CHECK(k >= 1 && k <= 16 && k <= K && K <= MAX_SLOTS && n <= MAX_SLOTS,
-              "tdc.topk_gate: 1 to 16 of the clusters, got k = ", k, " of ", K);
+  TORCH_CHECK_VALUE(k >= 1 && k <= std::min<int64_t>(16, K), "k must be 1 to ",
+                    std::min<int64_t>(16, K), ", got ", k);
+  TORCH_CHECK_VALUE(K <= MAX_SLOTS && n <= MAX_SLOTS, "too many scores: ", scores.sizes());
   const MaskArg m = mask_of(mask, scores, n, K);
   const DevGuard guard(scores.device());
   Tensor w = at::empty({n, k}, scores.options().dtype(at::kFloat));
@@ -246,13 +259,16 @@ Tensor gate_bwd_impl(const OptTensor& scores, const OptTensor& mask, const Tenso
 }
 
 // ------------------------------------------------------------------ groups
-std::vector<Tensor> group_plan(const Tensor& labels, int64_t K) {
-  TORCH_CHECK(labels.is_cuda() && labels.is_contiguous() &&
-                  (labels.scalar_type() == at::kInt || labels.scalar_type() == at::kLong),
-              "tdc.group_plan: labels must be contiguous int32 or int64 on the GPU");
-  const int64_t m = labels.numel();
-  TORCH_CHECK(K >= 1 && K < (1 << 22), "tdc.group_plan: 1 to 2^22 - 1 clusters, got ", K);
-  TORCH_CHECK(m <= MAX_SLOTS, "tdc.group_plan: too many labels: ", m);
+std::vector<Tensor> group_plan(const Tensor& given, int64_t K) {
+  TORCH_CHECK_VALUE((given.dim() == 1 || given.dim() == 2) &&
+                        (given.scalar_type() == at::kInt || given.scalar_type() == at::kLong),
+                    "labels must be int32 or int64 [N] or [N, k], got ", given.scalar_type(), " ",
+                    given.sizes());
+  TORCH_CHECK_VALUE(given.dim() == 1 || given.size(1) >= 1, "labels have no columns");
+  TORCH_CHECK_VALUE(K >= 1 && K < (1 << 22), "n_clusters must be 1 to ", (1 << 22) - 1, ", got ", K);
+  const int64_t m = given.numel();
+  TORCH_CHECK_VALUE(m <= MAX_SLOTS, "at most ", MAX_SLOTS, " labels, got ", m);
+  const Tensor labels = given.contiguous();
   const DevGuard guard(labels.device());
   const auto opt = labels.options().dtype(at::kInt);
   Tensor offsets = at::empty({K + 1}, opt);
@@ -282,7 +298,8 @@ Tensor group_impl(const Tensor& x, const Tensor& offsets, const Tensor& pos) {
   check_rows(x, "x");
   const int64_t n = x.size(0), d = x.size(1), k = slots_of(offsets, pos, x);
   const int code = code_of(x.scalar_type(), "x");
-  TORCH_CHECK(pos.size(0) == n && d >= 1 && d <= MAX_SLOTS, "tdc.group_rows: rows do not fit the plan");
+  TORCH_CHECK_VALUE(pos.size(0) == n && d <= MAX_SLOTS, "the plan is of ", pos.size(0),
+                    " rows, x has ", n);
   const DevGuard guard(x.device());
   Tensor out = at::empty({n * k, d}, x.options());
   check(tdc_group_rows(code, x.data_ptr(), x.stride(0), n, (int)k, (int)d,
@@ -296,9 +313,10 @@ Tensor combine_impl(const Tensor& y, const Tensor& offsets, const Tensor& pos, c
   check_rows(y, "y");
   const int64_t n = pos.size(0), d = y.size(1), k = slots_of(offsets, pos, y);
   const int code = code_of(y.scalar_type(), "y");
-  TORCH_CHECK(y.size(0) == n * k && d >= 1 && d <= MAX_SLOTS, "tdc.combine_rows: rows do not fit the plan");
+  TORCH_CHECK_VALUE(y.size(0) == n * k && d <= MAX_SLOTS, "the plan is of ", n * k,
+                    " places, y has ", y.size(0), " rows");
   bool w32;
-  const void* wp = weights_of(w, y, n * k, w32);
+  const void* wp = weights_of(w, y, pos.sizes(), "weights", w32);
   const DevGuard guard(y.device());
   Tensor out = at::empty({n, d}, y.options());
   check(tdc_combine_rows(code, y.data_ptr(), y.stride(0), n, (int)k, (int)d,
@@ -317,7 +335,7 @@ std::vector<Tensor> combine_bwd_impl(const Tensor& dout, const OptTensor& y, con
   TORCH_CHECK(pos.size(0) == n && d >= 1 && d <= MAX_SLOTS,
               "tdc.combine_rows_bwd: rows do not fit the plan");
   bool w32;
-  const void* wp = weights_of(w, dout, n * k, w32);
+  const void* wp = weights_of(w, dout, pos.sizes(), "weights", w32);
   const bool want_dw = has(y);
   if (want_dw) {
     check_rows(*y, "y");

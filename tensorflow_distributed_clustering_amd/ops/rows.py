@@ -42,9 +42,21 @@ def _ops():
     return _tdc
 
 
+def _on_gpu(**tensors) -> bool:
+    """Whether the kernels take the call.  Their bindings check its arguments themselves, with
+    the errors of the checks below, which are the CPU path's: a request pays for one set."""
+    gpu = None
+    for name, t in tensors.items():
+        if t is None and gpu is not None:
+            continue
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
+        if gpu is None:
+            gpu = t.is_cuda
+    return gpu
+
+
 def _check_rows(x, name: str):
-    if not isinstance(x, torch.Tensor):
-        raise TypeError(f"{name} must be a tensor, got {type(x).__name__}")
     if x.dim() != 2 or x.dtype not in ROW_DTYPES:
         raise ValueError(f"{name} must be fp32, fp16 or bf16 rows [N, D], got {x.dtype} {tuple(x.shape)}")
     if x.shape[1] < 1:
@@ -54,8 +66,6 @@ def _check_rows(x, name: str):
 
 
 def _check_weight(w, x, shape, name: str):
-    if not isinstance(w, torch.Tensor):
-        raise TypeError(f"{name} must be a tensor, got {type(w).__name__}")
     if tuple(w.shape) != tuple(shape) or not w.is_contiguous():
         raise ValueError(f"{name} must be contiguous {tuple(shape)}, got {tuple(w.shape)}")
     if w.dtype not in (torch.float32, x.dtype):
@@ -88,8 +98,8 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
     [D] is fp32 or of the rows' type (None: ones).  The squares are summed in fp32: a row
     whose sum of squares passes 3.4e38 becomes zeros.  With ``eps`` = 0 a row of zeros
     becomes NaN."""
-    _check_norm(x, weight, residual, eps)
-    if x.device.type != "cuda":
+    if not _on_gpu(x=x, weight=weight, residual=residual):
+        _check_norm(x, weight, residual, eps)
         return ref.rms_norm(x, weight, residual, eps)
     out = _ops().rms_norm(x, weight, residual, eps)
     return out[0] if residual is None else (out[0], out[1])
@@ -136,11 +146,13 @@ def rms_norm_fp8(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
     """:func:`rms_norm` whose ``y`` is computed in fp64 and rounded once to
     :class:`Fp8Rows`, one exponent per 32 columns.  Returns the rows, or ``(rows, h)`` with a residual.  For
     serving: it has no gradient, and refuses inputs that ask for one."""
-    _check_norm(x, weight, residual, eps)
+    gpu = _on_gpu(x=x, weight=weight, residual=residual)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
         raise RuntimeError("rms_norm_fp8 has no gradient: call it under torch.no_grad()")
+    if not gpu or x.dim() != 2:
+        _check_norm(x, weight, residual, eps)
     d = x.shape[1]
-    if x.device.type != "cuda":
+    if not gpu:
         out = ref.rms_norm_fp8(x, weight, residual, eps, fp8_width(d))
     else:
         out = _ops().rms_norm_fp8(x, weight, residual, eps, fp8_width(d))
@@ -160,25 +172,25 @@ def topk_gate(scores: torch.Tensor, k: int, mask: Optional[torch.Tensor] = None,
     never chosen, its score is not looked at and its gradient is zero.  Where fewer than k
     are left the last labels are -1 with weight 0, which :func:`group_plan` leaves out.  A
     NaN or +inf among the allowed scores makes the row's weights NaN."""
+    gpu = _on_gpu(scores=scores, mask=mask)
+    k, normalize = int(k), bool(normalize)
+    if mask is not None and mask.shape != scores.shape:
+        try:
+            mask = mask.expand(scores.shape)
+        except RuntimeError:
+            raise ValueError(f"mask {tuple(mask.shape)} does not broadcast to "
+                             f"{tuple(scores.shape)}") from None
+    if gpu:
+        return _ops().topk_gate(scores, mask, k, normalize)
     _check_rows(scores, "scores")
-    k = int(k)
     if not 1 <= k <= min(MAX_CHOSEN, scores.shape[1]):
         raise ValueError(f"k must be 1 to {min(MAX_CHOSEN, scores.shape[1])}, got {k}")
     if mask is not None:
-        if not isinstance(mask, torch.Tensor) or mask.dtype != torch.bool:
+        if mask.dtype != torch.bool:
             raise ValueError("mask must be a bool tensor")
         if mask.device != scores.device:
             raise ValueError(f"mask is on {mask.device}, the scores on {scores.device}")
-        if mask.shape != scores.shape:
-            try:
-                mask = mask.expand(scores.shape)
-            except RuntimeError:
-                raise ValueError(f"mask {tuple(mask.shape)} does not broadcast to "
-                                 f"{tuple(scores.shape)}") from None
-    normalize = bool(normalize)
-    if scores.device.type != "cuda":
-        return ref.topk_gate(scores, k, mask, normalize)
-    return _ops().topk_gate(scores, mask, k, normalize)
+    return ref.topk_gate(scores, k, mask, normalize)
 
 
 # ----------------------------------------------------------------- groups
@@ -213,21 +225,19 @@ def group_plan(labels: torch.Tensor, n_clusters: int) -> RowGroups:
     """Plan of the rows with ``labels`` (int32 or int64, [N] or [N, k]: k clusters per row)
     sorted by cluster; rows of one cluster keep their order.  Labels outside
     [0, n_clusters) drop their slot.  The same labels give the same plan."""
-    if not isinstance(labels, torch.Tensor):
-        raise TypeError(f"labels must be a tensor, got {type(labels).__name__}")
+    n_clusters = int(n_clusters)
+    if _on_gpu(labels=labels):
+        return RowGroups(*_ops().group_plan(labels, n_clusters), n_clusters)
     if labels.dim() not in (1, 2) or labels.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"labels must be int32 or int64 [N] or [N, k], got {labels.dtype} "
                          f"{tuple(labels.shape)}")
     if labels.dim() == 2 and labels.shape[1] < 1:
         raise ValueError("labels have no columns")
-    n_clusters = int(n_clusters)
     if not 1 <= n_clusters <= MAX_GROUPS:
         raise ValueError(f"n_clusters must be 1 to {MAX_GROUPS}, got {n_clusters}")
     if labels.numel() > MAX_SLOTS:
         raise ValueError(f"at most {MAX_SLOTS} labels, got {labels.numel()}")
-    if labels.device.type != "cuda":
-        return RowGroups(*ref.group_plan(labels, n_clusters), n_clusters)
-    return RowGroups(*_ops().group_plan(labels.contiguous(), n_clusters), n_clusters)
+    return RowGroups(*ref.group_plan(labels, n_clusters), n_clusters)
 
 
 def _check_groups(groups):
@@ -239,14 +249,14 @@ def group_rows(x: torch.Tensor, groups: RowGroups) -> torch.Tensor:
     """The rows of ``x`` [N, D] sorted by cluster, [N * k, D]: a row once for each of its
     labels, zeros at the places from ``groups.offsets[-1]`` on.  The gradient sums a row's
     copies in fp32."""
-    _check_rows(x, "x")
     _check_groups(groups)
+    if _on_gpu(x=x):
+        return _ops().group_rows(x, groups.offsets, groups.pos)
+    _check_rows(x, "x")
     if x.shape[0] != groups.n_rows or x.device != groups.pos.device:
         raise ValueError(f"the plan is of {groups.n_rows} rows on {groups.pos.device}, "
                          f"x has {x.shape[0]} on {x.device}")
-    if x.device.type != "cuda":
-        return ref.group_rows(x, groups.offsets, groups.order, groups.pos)
-    return _ops().group_rows(x, groups.offsets, groups.pos)
+    return ref.group_rows(x, groups.offsets, groups.order, groups.pos)
 
 
 def combine_rows(y: torch.Tensor, groups: RowGroups, weights: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -254,13 +264,13 @@ def combine_rows(y: torch.Tensor, groups: RowGroups, weights: Optional[torch.Ten
     y[place of slot (n, j)]``, in fp32 in the order of j and rounded once.  ``weights`` have
     the shape of the plan's labels, fp32 or of the rows' type (None: ones).  Slots without a
     cluster add nothing, whatever ``y`` holds there; a row that has none left is zeros."""
-    _check_rows(y, "y")
     _check_groups(groups)
+    if _on_gpu(y=y, weights=weights):
+        return _ops().combine_rows(y, groups.offsets, groups.pos, weights)
+    _check_rows(y, "y")
     if y.shape[0] != groups.n_slots or y.device != groups.pos.device:
         raise ValueError(f"the plan is of {groups.n_slots} places on {groups.pos.device}, "
                          f"y has {y.shape[0]} rows on {y.device}")
     if weights is not None:
         _check_weight(weights, y, groups.pos.shape, "weights")
-    if y.device.type != "cuda":
-        return ref.combine_rows(y, groups.offsets, groups.pos, weights)
-    return _ops().combine_rows(y, groups.offsets, groups.pos, weights)
+    return ref.combine_rows(y, groups.offsets, groups.pos, weights)

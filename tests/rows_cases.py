@@ -6,6 +6,9 @@ less; SUM covers widths to 16384 with tree sums (log2 n + a few roundings, taken
 """
 import torch
 
+import tensorflow_distributed_clustering_amd as tdc
+from tensorflow_distributed_clustering_amd.ops import rows as R
+
 DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 
 
@@ -105,3 +108,48 @@ def plan(labels, clusters):
         torch.searchsorted(torch.tensor(sorted(key)), torch.arange(clusters + 1)).tolist()
     t = lambda v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
     return t(offsets), t(order), t(pos).view(labels.shape)
+
+
+# calls that are refused, on rows x [4, 8] and labels l [4] of either device
+REFUSALS = {
+    "norm list": (lambda x, l: tdc.rms_norm([1.0]), TypeError),
+    "norm 1-D": (lambda x, l: tdc.rms_norm(x[0]), ValueError),
+    "norm fp64": (lambda x, l: tdc.rms_norm(x.double()), ValueError),
+    "norm columns": (lambda x, l: tdc.rms_norm(x.t()), ValueError),
+    "norm no columns": (lambda x, l: tdc.rms_norm(x[:, :0]), ValueError),
+    "norm too wide": (lambda x, l: tdc.rms_norm(x.new_zeros(1, R.MAX_WIDTH + 1)), ValueError),
+    "norm weight list": (lambda x, l: tdc.rms_norm(x, [1.0] * 8), TypeError),
+    "norm weight short": (lambda x, l: tdc.rms_norm(x, x.new_ones(7)), ValueError),
+    "norm weight type": (lambda x, l: tdc.rms_norm(x, x.new_ones(8).half()), ValueError),
+    "norm weight strided": (lambda x, l: tdc.rms_norm(x, x.new_ones(16)[::2]), ValueError),
+    "norm weight 2-D": (lambda x, l: tdc.rms_norm(x, x.new_ones(1, 8)), ValueError),
+    "norm residual type": (lambda x, l: tdc.rms_norm(x, residual=x.half()), ValueError),
+    "norm residual rows": (lambda x, l: tdc.rms_norm(x, residual=x[:3]), ValueError),
+    "norm residual columns": (lambda x, l: tdc.rms_norm(x[:, :4], residual=x.t()[:4]), ValueError),
+    "norm eps negative": (lambda x, l: tdc.rms_norm(x, eps=-1.0), ValueError),
+    "norm eps nan": (lambda x, l: tdc.rms_norm(x, eps=float("nan")), ValueError),
+    "fp8 gradient": (lambda x, l: tdc.rms_norm_fp8(x.clone().requires_grad_()), RuntimeError),
+    "fp8 1-D": (lambda x, l: tdc.rms_norm_fp8(x[0]), ValueError),
+    "fp8 too wide": (lambda x, l: tdc.rms_norm_fp8(x.new_zeros(1, R.MAX_WIDTH + 1)), ValueError),
+    "fp8 to fp64": (lambda x, l: tdc.rms_norm_fp8(x).dequantize(torch.float64), ValueError),
+    "gate k 0": (lambda x, l: tdc.topk_gate(x, 0), ValueError),
+    "gate k above clusters": (lambda x, l: tdc.topk_gate(x, 9), ValueError),
+    "gate k 17": (lambda x, l: tdc.topk_gate(x.new_zeros(2, 40), 17), ValueError),
+    "gate scores": (lambda x, l: tdc.topk_gate(l, 2), ValueError),
+    "gate mask type": (lambda x, l: tdc.topk_gate(x, 2, mask=x), ValueError),
+    "gate mask shape": (lambda x, l: tdc.topk_gate(x, 2, mask=x[:3] == 0), ValueError),
+    "gate mask list": (lambda x, l: tdc.topk_gate(x, 2, mask=[True] * 8), TypeError),
+    "plan list": (lambda x, l: tdc.group_plan([1], 2), TypeError),
+    "plan floats": (lambda x, l: tdc.group_plan(x, 2), ValueError),
+    "plan 3-D": (lambda x, l: tdc.group_plan(l[:, None, None], 2), ValueError),
+    "plan no columns": (lambda x, l: tdc.group_plan(l[:, None][:, :0], 2), ValueError),
+    "plan no clusters": (lambda x, l: tdc.group_plan(l, 0), ValueError),
+    "plan too many clusters": (lambda x, l: tdc.group_plan(l, R.MAX_GROUPS + 1), ValueError),
+    "group no plan": (lambda x, l: tdc.group_rows(x, None), TypeError),
+    "group rows": (lambda x, l: tdc.group_rows(x, tdc.group_plan(l[:3], 2)), ValueError),
+    "group type": (lambda x, l: tdc.group_rows(x.double(), tdc.group_plan(l, 2)), ValueError),
+    "combine rows": (lambda x, l: tdc.combine_rows(x, tdc.group_plan(l[:3], 2)), ValueError),
+    "combine weights shape": (lambda x, l: tdc.combine_rows(x, tdc.group_plan(l, 2), x.new_ones(4, 1)), ValueError),
+    "combine weights type": (lambda x, l: tdc.combine_rows(x, tdc.group_plan(l, 2), x.new_ones(4).double()), ValueError),
+    "combine weights list": (lambda x, l: tdc.combine_rows(x, tdc.group_plan(l, 2), [1.0] * 4), TypeError),
+}

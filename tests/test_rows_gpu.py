@@ -274,6 +274,27 @@ def test_group_and_combine(gpu, n, k, d, dtype):
             assert torch.equal(only, grads[1])
 
 
+# ----------------------------------------------------------------- refusals
+@pytest.mark.parametrize("name", rc.REFUSALS)
+def test_refusals(gpu, name):
+    call, error = rc.REFUSALS[name]
+    with pytest.raises(error):
+        call(torch.zeros(4, 8, device=gpu), torch.zeros(4, dtype=torch.int32, device=gpu))
+
+
+def test_refusals_of_another_device(gpu):
+    x, lab = torch.zeros(4, 8, device=gpu), torch.zeros(4, dtype=torch.int32, device=gpu)
+    groups = tdc.group_plan(lab, 2)
+    for call in (lambda: tdc.rms_norm(x, torch.ones(8)), lambda: tdc.rms_norm(x, residual=x.cpu()),
+                 lambda: tdc.rms_norm(x.cpu(), torch.ones(8, device=gpu)),
+                 lambda: tdc.topk_gate(x, 2, mask=(x == 0).cpu()), lambda: tdc.group_rows(x.cpu(), groups),
+                 lambda: tdc.combine_rows(x.cpu(), groups), lambda: tdc.group_rows(x, tdc.group_plan(lab.cpu(), 2)),
+                 lambda: tdc.combine_rows(x, groups, torch.ones(4)),
+                 lambda: tdc.ClusterPredictor(x[:2], dtype="fp8", device=gpu).predict(tdc.rms_norm_fp8(x.cpu()))):
+        with pytest.raises(ValueError):
+            call()
+
+
 # ----------------------------------------------------------------- large, streams
 def test_offsets_past_32_bits(gpu):
     n, d = 140_000, 16384                            # 2.29e9 elements
