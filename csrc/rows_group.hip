@@ -217,12 +217,15 @@ __global__ __launch_bounds__(SORT_BLOCK) void sort_scatter_kernel(
       // the last lane of the digit moves its next place on, after all have read it
       __builtin_amdgcn_wave_barrier();
       if ((same >> lane) == 1ull) *next = p + 1;
-      pos[slot_at] = p;  // of what stood here before the pass
-      if constexpr (LAST) {
-        order[p] = in.slot(slot_at);
-        if (keys) keys[p] = key[i];
-      } else {
-        pairs[p] = make_int2(key[i], in.slot(slot_at));
+      // always, unless someone writes the labels meanwhile
+      if ((unsigned)p < (unsigned)m) {
+        pos[slot_at] = p;  // of what stood here before the pass
+        if constexpr (LAST) {
+          order[p] = in.slot(slot_at);
+          if (keys) keys[p] = key[i];
+        } else {
+          pairs[p] = make_int2(key[i], in.slot(slot_at));
+        }
       }
     }
     __builtin_amdgcn_wave_barrier();
@@ -232,29 +235,24 @@ __global__ __launch_bounds__(SORT_BLOCK) void sort_scatter_kernel(
 // The end of a sort in two passes.  pos[slot] holds the place after the first pass, `moved`
 // where the second put what stood there: the slot's place is read through both (1M labels:
 // 18 us for the second pass and 11 here; 31 and 5 where that pass wrote pos[slot] itself, 4
-// bytes at a time all over).
-// offsets[c] = first place whose key is c or more, for c in 0..K: the places where the key
-// steps up write those they step over, a whole wave at a time.
+// bytes at a time all over).  offsets[c] is the first place whose key is c or more, looked
+// up by halving: as long for clusters that are all empty as for full ones.
 __global__ __launch_bounds__(SORT_BLOCK) void sort_finish_kernel(const int* __restrict__ keys,
                                                                  const int* __restrict__ moved,
                                                                  int m, int K, int* __restrict__ pos,
                                                                  int* __restrict__ offsets) {
-  const int lane = threadIdx.x & 63;
-  const int64_t p = (int64_t)blockIdx.x * SORT_BLOCK + threadIdx.x;
-  if (p < m) pos[p] = moved[pos[p]];
-  int lo = 0, hi = 0;  // this place writes offsets lo .. hi - 1
-  if (p <= m) {
-    lo = p == 0 ? 0 : keys[p - 1] + 1;
-    hi = p == m ? K + 1 : keys[p] + 1;
+  const int64_t i = (int64_t)blockIdx.x * SORT_BLOCK + threadIdx.x;
+  if (i < m) pos[i] = moved[min((unsigned)pos[i], (unsigned)m - 1)];
+  if (i > K) return;
+  int lo = 0, hi = m;
+  while (lo < hi) {
+    const int mid = lo + (hi - lo) / 2;
+    if (keys[mid] < i)
+      lo = mid + 1;
+    else
+      hi = mid;
   }
-  unsigned long long todo = __ballot(hi > lo);
-  while (todo) {
-    const int l = __ffsll((long long)todo) - 1;
-    todo &= todo - 1;
-    const int a = __shfl(lo, l, 64), b = __shfl(hi, l, 64);
-    const int place = __shfl((int)p, l, 64);
-    for (int c = a + lane; c < b; c += 64) offsets[c] = place;
-  }
+  offsets[i] = lo;
 }
 
 // ------------------------------------------------------------------ rows
@@ -548,7 +546,7 @@ struct SortShape {
     low = bits <= DIGIT_BITS ? bits : (bits + 1) / 2;
     high = bits - low;
     if (m <= SORT_BLOCK * 16)
-      per = 16;
+      per = m <= SORT_BLOCK * 4 ? 4 : m <= SORT_BLOCK * 8 ? 8 : 16;
     else
       per = m <= SORT_BLOCK * 4 * DIRECT_CHUNKS ? 4 : m <= (4 << 20) ? 8 : 16;
     chunks = std::max<int64_t>(1, (m + SORT_BLOCK * per - 1) / (SORT_BLOCK * per));
@@ -610,7 +608,8 @@ int tdc_group_plan(int wide_labels, const void* labels, int64_t m, int K, int* w
       if (rc == 0) rc = pass(FromPairs{pairs}, std::true_type(), per, s.low, s.high, s.digits[1]);
       if (rc) return rc;
     }
-    hipLaunchKernelGGL(sort_finish_kernel, dim3((unsigned)((m + 1 + SORT_BLOCK - 1) / SORT_BLOCK)),
+    const int64_t items = std::max<int64_t>(m, K + 1);
+    hipLaunchKernelGGL(sort_finish_kernel, dim3((unsigned)((items + SORT_BLOCK - 1) / SORT_BLOCK)),
                        block, 0, stream, keys, moved, (int)m, K, pos, offsets);
     TDC_CHECK_LAUNCH();
     return 0;

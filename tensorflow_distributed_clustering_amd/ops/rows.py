@@ -24,7 +24,7 @@ from typing import Optional, Tuple
 import torch
 
 from .. import _native
-from . import reference as ref
+from . import fp8_dim, reference as ref
 
 ROW_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 MAX_WIDTH = 16384            # columns of a normalised row
@@ -135,10 +135,7 @@ class Fp8Rows:
 def fp8_width(d: int) -> int:
     """Columns that ``d`` take as an fp8 operand: the widths of the fp8 assignment up to
     1024, then whole blocks of 32."""
-    for p in (256, 512, 768, 1024):
-        if d <= p:
-            return p
-    return (d + 31) // 32 * 32
+    return fp8_dim(d) or (d + 31) // 32 * 32
 
 
 def rms_norm_fp8(x: torch.Tensor, weight: Optional[torch.Tensor] = None,

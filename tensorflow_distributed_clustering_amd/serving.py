@@ -128,9 +128,10 @@ class ClusterPredictor:
     def partition(self, x):
         """The rows of ``x`` [B, D] (fp32, fp16 or bf16) sorted by their cluster, and the
         :class:`RowGroups` that say which rows those are: ``rows[groups.offsets[c] :
-        groups.offsets[c + 1]]`` are cluster c's, in their order in ``x``."""
+        groups.offsets[c + 1]]`` are cluster c's, in their order in ``x``.  Differentiable in
+        the rows (not in their cluster)."""
         x = torch.as_tensor(x).to(self.device)
-        groups = group_plan(self.predict(x), self.k)
+        groups = group_plan(self.predict(x.detach()), self.k)
         return group_rows(x, groups), groups
 
     def score(self, x) -> float:

@@ -163,7 +163,10 @@ def test_predictor_fp8_rows_and_partition():
         tdc.ClusterPredictor(c, dtype="fp32", device="cpu").predict(rows)
     with pytest.raises(ValueError):
         p.predict(tdc.rms_norm_fp8(x[:, :39].contiguous()))
+    x.requires_grad_()
     parts, groups = p.partition(x)
+    assert torch.equal(torch.autograd.grad(parts.sum(), x)[0], torch.ones_like(x))
+    x = x.detach()
     lab = p.predict(x)
     for k in range(9):
         at = groups.offsets[k:k + 2].tolist()

@@ -204,7 +204,8 @@ def test_gate_nan_and_inf_that_are_allowed(gpu):
 # ----------------------------------------------------------------- plan, group, combine
 @pytest.mark.parametrize("n,k,clusters", [(0, 2, 4), (1, 1, 1), (8, 2, 64), (4096, 1, 7), (4097, 1, 2047),
                                           (1500, 8, 256), (100, 1, 2048), (30000, 2, 65536),
-                                          (0, 1, 70000), (5000, 1, 300000), (70001, 3, 33)])
+                                          (0, 1, 70000), (5000, 1, 300000), (70001, 3, 33),
+                                          (300000, 1, 257), (3, 1, (1 << 22) - 1)])
 @pytest.mark.parametrize("wide", [False, True])
 def test_plan(gpu, n, k, clusters, wide):
     g = torch.Generator().manual_seed(n + clusters)
