@@ -270,7 +270,17 @@ __device__ __forceinline__ int kept_places(const int* offsets, int K, int64_t m)
 template <typename T, bool SHORT> __device__ __forceinline__ Raw16 take(const T* row, int c, int d) {
   return RowVec<T, SHORT ? TAIL_SHORT : TAIL_NONE>::fetch(row, c, d);
 }
-template <typename T, bool SHORT>
+// f(STREAM): whether the sorted rows are stored past the caches: where they are as large as the last
+// level (256 MiB) they would only push out what the next kernel reads, and still be on their
+// way to memory then (131072 x 1024 bf16: grouped and the gradient summed 134 us past the
+// caches, 154 through them; grouped and read 422 us either way).  Smaller ones are kept for
+// their reader (64 MiB grouped and read: 104 us past the caches, 85 through them).
+template <typename F> int with_stream(int64_t bytes, F&& f) {
+  if (bytes >= (int64_t)256 << 20) return f(std::true_type());
+  return f(std::false_type());
+}
+
+template <typename T, bool SHORT, bool STREAM = false>
 __device__ __forceinline__ void put(T* row, int c, int d, const Raw16& r) {
   if constexpr (SHORT) {
     T t[Vec<T>::N];
@@ -279,7 +289,14 @@ __device__ __forceinline__ void put(T* row, int c, int d, const Raw16& r) {
     for (int i = 0; i < Vec<T>::N; ++i)
       if (c + i < d) row[c + i] = t[i];
   } else {
-    store16(row + min(c, d - Vec<T>::N), r);
+    T* p = row + min(c, d - Vec<T>::N);
+    if constexpr (STREAM) {
+      typedef unsigned Words __attribute__((ext_vector_type(4), aligned(2)));
+      const Words v = {r.w[0], r.w[1], r.w[2], r.w[3]};
+      __builtin_nontemporal_store(v, reinterpret_cast<Words*>(p));
+    } else {
+      store16(p, r);
+    }
   }
 }
 
@@ -301,7 +318,7 @@ __device__ __forceinline__ bool piece(int u, int L, int64_t n, int d, int pass, 
 // kept ones), J slots at a time: their places are all there before the first store, as a
 // wait for a load waits for the stores before it too (rows of 2 KiB with k = 8: 6.4 TB/s,
 // 3.5 with a place fetched before each store).
-template <typename T, int J, int U, bool LONG, bool SHORT>
+template <typename T, int J, int U, bool LONG, bool SHORT, bool STREAM>
 __global__ __launch_bounds__(256) void group_kernel(const T* __restrict__ x, int64_t ldx, int64_t n,
                                                     int k, int d, const int* __restrict__ offsets,
                                                     int K, const int* __restrict__ pos,
@@ -331,7 +348,7 @@ __global__ __launch_bounds__(256) void group_kernel(const T* __restrict__ x, int
 #pragma unroll
       for (int j = 0; j < J; ++j)
         if ((unsigned)p[u][j] < (unsigned)(n * k))
-          put<T, SHORT>(out + (int64_t)p[u][j] * d, c[u], d, if_kept(p[u][j] < kept, v[u]));
+          put<T, SHORT, STREAM>(out + (int64_t)p[u][j] * d, c[u], d, if_kept(p[u][j] < kept, v[u]));
   }
 }
 
@@ -401,7 +418,7 @@ __global__ __launch_bounds__(256) void combine_kernel(const T* __restrict__ y, i
 // Gradients of a row's slots, J at a time: dy[p] = w dout[row], dw = <dout[row], y[p]>;
 // either may be left out (dy null, y null).  The row's passes and the sum over its lanes
 // are this thread group's, so dw needs no atomics.
-template <typename T, int J, int U, bool LONG, bool SHORT>
+template <typename T, int J, int U, bool LONG, bool SHORT, bool STREAM>
 __global__ __launch_bounds__(256) void combine_bwd_kernel(
     const T* __restrict__ dout, int64_t lddo, const T* __restrict__ y, int64_t ldy, int64_t n, int k,
     int d, const int* __restrict__ offsets, int K, const int* __restrict__ pos,
@@ -463,7 +480,7 @@ __global__ __launch_bounds__(256) void combine_bwd_kernel(
             float o[N];
 #pragma unroll
             for (int i = 0; i < N; ++i) o[i] = ww * f[i];
-            put<T, SHORT>(dy + (int64_t)at * d, c[u], d, if_kept(at < kept, pack<T>(o)));
+            put<T, SHORT, STREAM>(dy + (int64_t)at * d, c[u], d, if_kept(at < kept, pack<T>(o)));
           }
           if (y && in[u] && at < kept) {
             float q[N];
@@ -636,10 +653,13 @@ int tdc_group_rows(int dtype, const void* x, int64_t ldx, int64_t n, int k, int 
         constexpr int J = decltype(jj)::value, U = decltype(uu)::value;
         dim3 grid;
         if (!grid_for(n, d, V, L, U, LONG, true, grid)) return (int)hipErrorInvalidValue;
-        hipLaunchKernelGGL((group_kernel<T, J, U, LONG, SHORT>), grid, dim3(256), 0, stream,
-                           (const T*)x, ldx, n, k, d, offsets, K, pos, (T*)out, L);
-        TDC_CHECK_LAUNCH();
-        return 0;
+        return with_stream(n * k * d * (int64_t)sizeof(T), [&](auto past) {
+          constexpr bool STREAM = decltype(past)::value;
+          hipLaunchKernelGGL((group_kernel<T, J, U, LONG, SHORT, STREAM>), grid, dim3(256), 0, stream,
+                             (const T*)x, ldx, n, k, d, offsets, K, pos, (T*)out, L);
+          TDC_CHECK_LAUNCH();
+          return 0;
+        });
       });
     });
   });
@@ -682,11 +702,14 @@ int tdc_combine_rows_bwd(int dtype, const void* dout, int64_t lddo, const void* 
         constexpr int J = decltype(jj)::value, U = decltype(uu)::value;
         dim3 grid;
         if (!grid_for(n, d, V, L, U, LONG, false, grid)) return (int)hipErrorInvalidValue;
-        hipLaunchKernelGGL((combine_bwd_kernel<T, J, U, LONG, SHORT>), grid, dim3(256), 0, stream,
-                           (const T*)dout, lddo, (const T*)y, ldy, n, k, d, offsets, K, pos, w,
-                           w32 != 0, (T*)dy, dw, L);
-        TDC_CHECK_LAUNCH();
-        return 0;
+        return with_stream(n * k * d * (int64_t)sizeof(T), [&](auto past) {
+          constexpr bool STREAM = decltype(past)::value;
+          hipLaunchKernelGGL((combine_bwd_kernel<T, J, U, LONG, SHORT, STREAM>), grid, dim3(256), 0,
+                             stream, (const T*)dout, lddo, (const T*)y, ldy, n, k, d, offsets, K,
+                             pos, w, w32 != 0, (T*)dy, dw, L);
+          TDC_CHECK_LAUNCH();
+          return 0;
+        });
       });
     });
   });
