@@ -27,6 +27,7 @@ hipStream_t cur_stream() { return at::hip::getCurrentHIPStreamMasqueradingAsCUDA
 
 constexpr int64_t MAX_WIDTH = 16384;
 constexpr int64_t MAX_SLOTS = std::numeric_limits<int32_t>::max() - 1;
+constexpr int64_t MAX_COLUMNS = 1 << 24;  // of grouped rows: passes over a row are grid blocks
 
 int code_of(at::ScalarType t, const char* what) {
   switch (t) {
@@ -298,8 +299,8 @@ Tensor group_impl(const Tensor& x, const Tensor& offsets, const Tensor& pos) {
   check_rows(x, "x");
   const int64_t n = x.size(0), d = x.size(1), k = slots_of(offsets, pos, x);
   const int code = code_of(x.scalar_type(), "x");
-  TORCH_CHECK_VALUE(pos.size(0) == n && d <= MAX_SLOTS, "the plan is of ", pos.size(0),
-                    " rows, x has ", n);
+  TORCH_CHECK_VALUE(pos.size(0) == n, "the plan is of ", pos.size(0), " rows, x has ", n);
+  TORCH_CHECK_VALUE(d <= MAX_COLUMNS, "at most ", MAX_COLUMNS, " columns, got ", d);
   const DevGuard guard(x.device());
   Tensor out = at::empty({n * k, d}, x.options());
   check(tdc_group_rows(code, x.data_ptr(), x.stride(0), n, (int)k, (int)d,
@@ -313,8 +314,9 @@ Tensor combine_impl(const Tensor& y, const Tensor& offsets, const Tensor& pos, c
   check_rows(y, "y");
   const int64_t n = pos.size(0), d = y.size(1), k = slots_of(offsets, pos, y);
   const int code = code_of(y.scalar_type(), "y");
-  TORCH_CHECK_VALUE(y.size(0) == n * k && d <= MAX_SLOTS, "the plan is of ", n * k,
-                    " places, y has ", y.size(0), " rows");
+  TORCH_CHECK_VALUE(y.size(0) == n * k, "the plan is of ", n * k, " places, y has ", y.size(0),
+                    " rows");
+  TORCH_CHECK_VALUE(d <= MAX_COLUMNS, "at most ", MAX_COLUMNS, " columns, got ", d);
   bool w32;
   const void* wp = weights_of(w, y, pos.sizes(), "weights", w32);
   const DevGuard guard(y.device());

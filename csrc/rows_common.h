@@ -53,8 +53,8 @@ template <typename T> __device__ __forceinline__ Raw16 pack(const float (&v)[Vec
 // How a row of `width` splits into vectors of N elements: TAIL_NONE: without rest;
 // TAIL_SHIFT: its last vector is partial; TAIL_SHORT: it is shorter than one vector.
 // A load must not sit in a branch of its own lanes: the wait for it would sit there too,
-// and the loads of a thread would go out one after the other (measured on rows of 2 KiB
-// moved by place: 3.5 TB/s with a branch around each load, 5.9 without).
+// and the loads of a thread would go out one after the other (the gradients of 131072 x 1024
+// combined bf16 rows took 202 us with a branch around each load, 111 without).
 enum Tail { TAIL_NONE = 0, TAIL_SHIFT = 1, TAIL_SHORT = 2 };
 
 // Elements [c, c + N) of a row; fetch() issues the load, value() gives the floats, 0 past
@@ -117,6 +117,17 @@ template <typename F> int with_tail(int d, int n, F&& f) {
   if (d < n) return f(std::integral_constant<int, TAIL_SHORT>());
   if (d % n) return f(std::integral_constant<int, TAIL_SHIFT>());
   return f(std::integral_constant<int, TAIL_NONE>());
+}
+
+// Blocks over two grid dimensions: a dimension times the block's threads has to stay below
+// 2^32, which one dimension alone does not for 17M rows of a block each.  Blocks past the
+// last row find nothing to do.
+inline dim3 grid_of(int64_t blocks, unsigned z = 1) {
+  const int64_t x = blocks < (1 << 21) ? blocks : (1 << 21);
+  return dim3((unsigned)x, (unsigned)((blocks + x - 1) / x), z);
+}
+__device__ __forceinline__ int64_t block_index() {
+  return (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
 }
 
 // The lane of this 16-lane row that DPP control CTRL names.

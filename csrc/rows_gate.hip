@@ -132,7 +132,7 @@ __global__ __launch_bounds__(GATE_BLOCK) void gate_kernel(const T* __restrict__ 
   __shared__ unsigned s_all[2][4];
   int turn = 0;
   const int lane = threadIdx.x % L;
-  const int64_t row = (int64_t)blockIdx.x * (GATE_BLOCK / L) + threadIdx.x / L;
+  const int64_t row = block_index() * (GATE_BLOCK / L) + threadIdx.x / L;
   if (row >= n) return;  // whole groups of 16; L >= 64: a whole wave or block
   const T* src = scores + row * ld;
   Raw16 raw[R / V];
@@ -256,7 +256,8 @@ __global__ __launch_bounds__(GATE_BLOCK) void gate_wide_kernel(
   __shared__ unsigned s_key[2][4];
   __shared__ int s_at[2][4];
   __shared__ float s_sum[4];
-  const int64_t row = blockIdx.x;
+  const int64_t row = block_index();
+  if (row >= n) return;
   const T* src = scores + row * ld;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   unsigned last = 0xffffffffu, mine = 0;
@@ -328,7 +329,7 @@ __global__ __launch_bounds__(GATE_BLOCK) void gate_bwd_kernel(
   __shared__ float more[GATE_BLOCK / L][PASS];
   const int lane = threadIdx.x % L;
   float* mine = more[threadIdx.x / L];
-  const int64_t row = (int64_t)blockIdx.x * (GATE_BLOCK / L) + threadIdx.x / L;
+  const int64_t row = block_index() * (GATE_BLOCK / L) + threadIdx.x / L;
   if (row >= n) return;
   const float wj = lane < k ? w[row * k + lane] : 0.f;
   const float dj = lane < k ? dw[row * k + lane] : 0.f;
@@ -390,7 +391,7 @@ int tdc_topk_gate(int dtype, const void* scores, int64_t ld, const uint8_t* mask
     using T = decltype(t);
     auto go = [&](auto kernel, int lanes) {
       const int rows = GATE_BLOCK / lanes;
-      hipLaunchKernelGGL(kernel, dim3((unsigned)((n + rows - 1) / rows)), dim3(GATE_BLOCK), 0,
+      hipLaunchKernelGGL(kernel, grid_of((n + rows - 1) / rows), dim3(GATE_BLOCK), 0,
                          stream, (const T*)scores, ld, m, n, K, k, normalize != 0, w, labels, stat);
     };
     return with_tail(K, Vec<T>::N, [&](auto tail) {
@@ -429,7 +430,7 @@ int tdc_topk_gate_bwd(int dtype, const void* scores, int64_t ld, const uint8_t* 
     using T = decltype(t);
     auto go = [&](auto kernel, int lanes) {
       const int rows = GATE_BLOCK / lanes;
-      hipLaunchKernelGGL(kernel, dim3((unsigned)((n + rows - 1) / rows)), dim3(GATE_BLOCK), 0,
+      hipLaunchKernelGGL(kernel, grid_of((n + rows - 1) / rows), dim3(GATE_BLOCK), 0,
                          stream, (const T*)scores, ld, m, w, labels, stat, dw, n, K, k,
                          normalize != 0, (T*)ds);
     };

@@ -327,6 +327,13 @@ def test_offsets_past_32_bits(gpu):
     rc.close(ds[-1:], want, torch.bfloat16, scale=torch.ones(1))
 
 
+def test_more_rows_than_one_grid_dimension_has_threads(gpu):
+    one = normal(gpu, 1, 1, 1100, dtype=torch.bfloat16)
+    n = 17_000_000                                   # a block of 256 threads each: over 2^32
+    w, lab = tdc.topk_gate(one.expand(n, 1100), 1)
+    assert lab.shape == (n, 1) and bool((lab == int(one.argmax())).all()) and bool((w == 1).all())
+
+
 def test_two_streams_at_once_and_inference_mode(gpu):
     x, w = normal(gpu, 1, 5000, 300, dtype=torch.bfloat16), normal(gpu, 2, 300)
     s = normal(gpu, 3, 5000, 40)
