@@ -148,18 +148,19 @@ __global__ __launch_bounds__(SORT_BLOCK) void sort_scatter_kernel(
       s_before[d] = hist[(int64_t)d * chunks + chunk];
     }
   } else if (chunks > 1) {
-    // each wave a quarter of the chunks, all of a digit's loads in flight
-    constexpr int PART = DIRECT_CHUNKS / SORT_WAVES;
-    for (int d = lane; d < digits; d += 64) {
-      int v[PART], t = 0, before = 0;
+    // pieces of 64 digits by 16 chunks, all of a piece's loads in flight: the counts come from
+    // other XCDs, a microsecond away.  The waves share the chunks first, then the digits.
+    constexpr int DEEP = DIRECT_CHUNKS / SORT_WAVES;
+    const int parts = chunks <= DEEP ? 1 : chunks <= 2 * DEEP ? 2 : SORT_WAVES;
+    const int c = (wave & (parts - 1)) * DEEP;
+    for (int d = wave / parts * 64 + lane; d < digits; d += SORT_WAVES / parts * 64) {
+      int v[DEEP], t = 0, before = 0;
 #pragma unroll
-      for (int i = 0; i < PART; ++i)
-        v[i] = hist[min(wave * PART + i, chunks - 1) * digits + d];
+      for (int i = 0; i < DEEP; ++i) v[i] = hist[min(c + i, chunks - 1) * digits + d];
 #pragma unroll
-      for (int i = 0; i < PART; ++i) {
-        const int c = wave * PART + i;
-        t += c < chunks ? v[i] : 0;
-        before += c < chunk ? v[i] : 0;
+      for (int i = 0; i < DEEP; ++i) {
+        t += c + i < chunks ? v[i] : 0;
+        before += c + i < chunk ? v[i] : 0;
       }
       atomicAdd(&s_total[d], t);
       atomicAdd(&s_before[d], before);
@@ -560,18 +561,21 @@ struct SortShape {
     while ((K >> bits) != 0) ++bits;  // keys 0..K
     low = bits <= DIGIT_BITS ? bits : (bits + 1) / 2;
     high = bits - low;
-    if (m <= SORT_BLOCK * 16)
-      per = m <= SORT_BLOCK * 4 ? 4 : m <= SORT_BLOCK * 8 ? 8 : 16;
+    if (m <= SORT_BLOCK * 8)
+      per = m <= SORT_BLOCK * 4 ? 4 : 8;
     else
-      per = m <= SORT_BLOCK * 4 * DIRECT_CHUNKS ? 4 : m <= (4 << 20) ? 8 : 16;
+      per = m <= SORT_BLOCK * 4 * DIRECT_CHUNKS ? 4 : m <= (2 << 20) ? 8 : 16;
     chunks = std::max<int64_t>(1, (m + SORT_BLOCK * per - 1) / (SORT_BLOCK * per));
     digits[0] = high ? 1 << low : K + 1;
     digits[1] = high ? (K >> low) + 1 : 0;
   }
   int64_t most() const { return std::max(digits[0], digits[1]); }
+  // Whether every block sums the chunks' counts itself, which saves a launch, or a kernel of
+  // its own does.
+  bool direct() const { return chunks <= DIRECT_CHUNKS && (most() <= 512 || chunks <= 16); }
   // counts of a pass, totals behind them, to whole int2
   int64_t count_words() const {
-    return chunks == 1 ? 0 : (most() * (chunks + (chunks > DIRECT_CHUNKS ? 1 : 0)) + 1) / 2 * 2;
+    return chunks == 1 ? 0 : (most() * (chunks + (direct() ? 0 : 1)) + 1) / 2 * 2;
   }
 };
 
@@ -591,7 +595,7 @@ int tdc_group_plan(int wide_labels, const void* labels, int64_t m, int K, int* w
   if (K < 1 || K >= (1 << 22) || m < 0 || m > 0x7ffffffe) return (int)hipErrorInvalidValue;
   const SortShape s(m, K);
   int* hist = s.chunks > 1 ? work : nullptr;
-  int* totals = s.chunks > DIRECT_CHUNKS ? work + s.most() * s.chunks : nullptr;
+  int* totals = s.chunks > 1 && !s.direct() ? work + s.most() * s.chunks : nullptr;
   int2* pairs = s.high ? reinterpret_cast<int2*>(work + s.count_words()) : nullptr;
   int* keys = s.high ? work + s.count_words() + 2 * m : nullptr;
   int* moved = s.high ? keys + m : nullptr;
