@@ -9,14 +9,19 @@
 // Scores are compared as whole numbers of the same order (0 = not to be chosen), so the
 // choice does not depend on any rounding; exp and the sums are fp32.
 //
-// Up to 4096 clusters a row stays in the registers of L threads, 16 scores each.  A score
-// and its index become one number, the index in place of the score's last 7 to 12 bits as
-// fp32: 16-bit types have nothing there.  The j-th choice is the largest number
+// Up to 8192 clusters a row stays in the registers of L threads, 8 to 32 scores each: as few
+// threads as hold it, since a round's part over the threads costs each of them the same (64M
+// bf16 scores, k = 8, in rows of 600: 54 us as 32 x 24, 78 as 64 x 16; in rows of 64: 60 us
+// as 8 x 8, 111 as 16 x 8).
+//
+// A score and its index become one number, the index in place of the score's last 6 to 13
+// bits as fp32: 16-bit types have nothing there.  The j-th choice is the largest number
 // below the (j-1)-th, found as the smallest of (limit - number), where what is above the
 // limit wraps around to more than the rest: 1.5 instructions per score and round, nothing
 // is taken out.  Where fp32 loses bits that are not zero and two neighbours among the first
 // k + 1 choices agree in the bits that are left, the rows of that wave are chosen again by
 // the whole scores.  65536 x 256 fp32, k = 8: 21 us, 37 with whole scores in every round.
+// Bound by these instructions from k = 4 or so, by memory below.
 #include "rows_common.h"
 
 namespace tdc {
@@ -85,8 +90,14 @@ template <typename Op> __device__ __forceinline__ unsigned row_all(unsigned v, O
 }
 template <int L, typename Op>
 __device__ __forceinline__ unsigned group_all(unsigned v, Op op, unsigned (*s)[4], int& turn) {
+  if constexpr (L == 8) {
+    v = op(v, dpp<DPP_XOR1>(v));
+    v = op(v, dpp<DPP_XOR2>(v));
+    return op(v, dpp<DPP_HALF_MIRROR>(v));
+  }
   v = row_all(v, op);
-  if constexpr (L > 16) {
+  if constexpr (L == 32) v = op(v, (unsigned)__shfl_xor((int)v, 16, 64));
+  if constexpr (L > 32) {
     v = op(op((unsigned)__builtin_amdgcn_readlane((int)v, 0),
               (unsigned)__builtin_amdgcn_readlane((int)v, 16)),
            op((unsigned)__builtin_amdgcn_readlane((int)v, 32),
@@ -116,6 +127,13 @@ struct Sum {
   }
 };
 
+// The fewest low bits, as a mask, that number n things.
+constexpr unsigned low_bits(int n) {
+  unsigned b = 1;
+  while ((int)b < n) b *= 2;
+  return b - 1;
+}
+
 template <int R> constexpr int column(int i, int v, int L, int lane) {
   return ((i / v) * L + lane) * v + i % v;
 }
@@ -127,13 +145,13 @@ __global__ __launch_bounds__(GATE_BLOCK) void gate_kernel(const T* __restrict__ 
                                                           int* __restrict__ labels,
                                                           float* __restrict__ stat) {
   constexpr int V = Vec<T>::N;
-  constexpr unsigned INDEX = L * R - 1;       // the bits of a column
+  constexpr unsigned INDEX = low_bits(L * R);  // the bits of a column
   constexpr unsigned NONE = 0x007fffffu;      // the place of -inf: it and less is not chosen
   __shared__ unsigned s_all[2][4];
   int turn = 0;
   const int lane = threadIdx.x % L;
   const int64_t row = block_index() * (GATE_BLOCK / L) + threadIdx.x / L;
-  if (row >= n) return;  // whole groups of 16; L >= 64: a whole wave or block
+  if (row >= n) return;  // whole groups of L; L >= 64: a whole wave or block
   const T* src = scores + row * ld;
   Raw16 raw[R / V];
   MaskVec<V, TAIL> ok[R / V];
@@ -398,14 +416,28 @@ int tdc_topk_gate(int dtype, const void* scores, int64_t ld, const uint8_t* mask
       constexpr int TAIL = decltype(tail)::value;
       auto one = [&](auto masked) {
         constexpr bool MASKED = decltype(masked)::value;
-        if (K <= 128)
+        if (K <= 64 && k <= 8)
+          go(gate_kernel<T, 8, 8, TAIL, MASKED>, 8);
+        else if (K <= 128)
           go(gate_kernel<T, 16, 8, TAIL, MASKED>, 16);
         else if (K <= 256)
           go(gate_kernel<T, 16, 16, TAIL, MASKED>, 16);
+        else if (K <= 384)
+          go(gate_kernel<T, 16, 24, TAIL, MASKED>, 16);
+        else if (K <= 512)
+          go(gate_kernel<T, 16, 32, TAIL, MASKED>, 16);
+        else if (K <= 768)
+          go(gate_kernel<T, 32, 24, TAIL, MASKED>, 32);
         else if (K <= 1024)
-          go(gate_kernel<T, 64, 16, TAIL, MASKED>, 64);
+          go(gate_kernel<T, 32, 32, TAIL, MASKED>, 32);
+        else if (K <= 1536)
+          go(gate_kernel<T, 64, 24, TAIL, MASKED>, 64);
+        else if (K <= 2048)
+          go(gate_kernel<T, 64, 32, TAIL, MASKED>, 64);
         else if (K <= 4096)
           go(gate_kernel<T, 256, 16, TAIL, MASKED>, 256);
+        else if (K <= 8192)
+          go(gate_kernel<T, 256, 32, TAIL, MASKED>, 256);
         else
           go(gate_wide_kernel<T>, GATE_BLOCK);
       };
@@ -438,6 +470,8 @@ int tdc_topk_gate_bwd(int dtype, const void* scores, int64_t ld, const uint8_t* 
       constexpr int TAIL = decltype(tail)::value;
       if (K <= 256)
         go(gate_bwd_kernel<T, 16, TAIL>, 16);
+      else if (K <= 512)
+        go(gate_bwd_kernel<T, 32, TAIL>, 32);
       else
         go(gate_bwd_kernel<T, 64, TAIL>, 64);
       TDC_CHECK_LAUNCH();

@@ -71,24 +71,24 @@ def fp8(y64, width):
 
 
 def gate(scores, k, mask, normalize, dw=None):
-    """(weights, labels[, ds]) with the choice made one by one, as Python compares."""
+    """(weights, labels[, ds]) row by row: NaN above +inf, equal scores by their index."""
     v = scores.double()
     n, clusters = v.shape
     ok = (v != -torch.inf) if mask is None else (mask.expand(v.shape) & (v != -torch.inf))
-    rank = torch.where(v.isnan(), torch.inf, v)
-    rank2 = v.isnan().double()                      # NaN orders above +inf
     weights = torch.zeros(n, k, dtype=torch.float64)
     labels = torch.full((n, k), -1, dtype=torch.int32)
     ds = torch.zeros(n, clusters, dtype=torch.float64)
     for r in range(n):
-        idx = [c for c in range(clusters) if bool(ok[r, c])]
-        pick = sorted(idx, key=lambda c: (-float(rank2[r, c]), -float(rank[r, c]), c))[:k]
-        if not pick:
+        idx = ok[r].nonzero().flatten()
+        nan = v[r, idx].isnan()
+        idx = torch.cat([idx[nan], idx[~nan][torch.sort(v[r, idx[~nan]], descending=True, stable=True)[1]]])
+        pick = idx[:k]
+        if not len(pick):
             continue
         of = pick if normalize else idx
         p = torch.zeros(clusters, dtype=torch.float64)
         p[of] = torch.softmax(v[r, of], 0)
-        labels[r, :len(pick)] = torch.tensor(pick, dtype=torch.int32)
+        labels[r, :len(pick)] = pick.int()
         weights[r, :len(pick)] = p[pick]
         if dw is not None:
             up = torch.zeros(clusters, dtype=torch.float64)

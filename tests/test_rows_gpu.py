@@ -140,8 +140,8 @@ def test_gradients_are_not_differentiable(gpu):
 
 
 # ----------------------------------------------------------------- gate
-@pytest.mark.parametrize("clusters,k", [(1, 1), (7, 7), (64, 2), (100, 16), (129, 3), (256, 8), (257, 6),
-                                        (1000, 8), (1024, 16), (1025, 5), (4099, 16)])
+@pytest.mark.parametrize("clusters,k", [(1, 1), (7, 7), (64, 2), (100, 16), (129, 3), (256, 8), (257, 6), (300, 9), (512, 7), (60, 8), (700, 16), (1500, 4),
+                                        (1000, 8), (1024, 16), (1025, 5), (4099, 16), (8192, 3), (8200, 5)])
 @pytest.mark.parametrize("dtype", rc.DTYPES)
 def test_gate(gpu, clusters, k, dtype):
     n = 11
