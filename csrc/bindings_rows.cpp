@@ -7,6 +7,7 @@
 #include <torch/extension.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <ATen/hip/HIPContext.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
@@ -42,6 +43,11 @@ int code_of(at::ScalarType t, const char* what) {
 void check(int err, const char* what) {
   TORCH_CHECK(err == 0, "tdc: ", what, " failed: ", hipGetErrorString((hipError_t)err), " (code ",
               err, ")");
+}
+
+// A new tensor on `like`'s device, without the dispatcher's rounds (0.4 us each).
+Tensor fresh(at::IntArrayRef sizes, at::ScalarType t, const Tensor& like) {
+  return at::detail::empty_cuda(sizes, t, like.device(), std::nullopt);
 }
 
 bool has(const OptTensor& t) { return t.has_value() && t->defined(); }
@@ -108,20 +114,20 @@ std::vector<Tensor> norm_impl(const Tensor& x, const OptTensor& w, const OptTens
   std::vector<Tensor> res;
   Tensor q, s, y;
   if (fp8_width) {
-    q = at::empty({n, fp8_width}, x.options().dtype(at::kFloat8_e4m3fn));
-    s = at::empty({n, fp8_width / 32}, x.options().dtype(at::kByte));
+    q = fresh({n, fp8_width}, at::kFloat8_e4m3fn, x);
+    s = fresh({n, fp8_width / 32}, at::kByte, x);
     res = {q, s};
   } else {
-    y = at::empty({n, d}, x.options());
+    y = fresh({n, d}, x.scalar_type(), x);
     res = {y};
   }
   Tensor h, rstd;
   if (has(r)) {
-    h = at::empty({n, d}, x.options());
+    h = fresh({n, d}, x.scalar_type(), x);
     res.push_back(h);
   }
   if (want_rstd) {
-    rstd = at::empty({n}, x.options().dtype(at::kFloat));
+    rstd = fresh({n}, at::kFloat, x);
     res.push_back(rstd);
   }
   check(tdc_rms_norm(code, x.data_ptr(), x.stride(0), has(r) ? r->data_ptr() : nullptr,
@@ -148,13 +154,13 @@ std::vector<Tensor> norm_bwd_impl(const Tensor& h, const OptTensor& w, const Ten
   bool w32;
   const void* wp = weights_of(w, h, {d}, "weight", w32);
   const DevGuard guard(h.device());
-  Tensor dx = at::empty({n, d}, h.options());
+  Tensor dx = fresh({n, d}, h.scalar_type(), h);
   std::vector<Tensor> res = {dx};
   Tensor part, dw;
   const int parts = tdc_rms_norm_bwd_parts(n, num_cus(h));
   if (want_dw) {
-    dw = at::empty({d}, w->options());
-    part = at::empty({parts, d}, h.options().dtype(at::kFloat));
+    dw = fresh({d}, w->scalar_type(), *w);
+    part = fresh({parts, d}, at::kFloat, h);
     res.push_back(dw);
   }
   check(tdc_rms_norm_bwd(code, h.data_ptr(), h.stride(0), rstd.data_ptr<float>(), wp, w32,
@@ -175,7 +181,7 @@ Tensor dequant_fp8(const Tensor& q, const Tensor& s, int64_t d, at::ScalarType d
                   s.numel() == q.size(0) * (q.size(1) / 32), "tdc.dequant_fp8: s uint8 [N, m]");
   const int code = code_of(dtype, "dtype");
   const DevGuard guard(q.device());
-  Tensor out = at::empty({q.size(0), d}, q.options().dtype(dtype));
+  Tensor out = fresh({q.size(0), d}, dtype, q);
   check(tdc_dequant_fp8(code, q.data_ptr(), s.data_ptr(), q.size(0), (int)d, (int)q.size(1),
                         out.data_ptr(), cur_stream()),
         "dequant_fp8");
@@ -212,12 +218,12 @@ std::vector<Tensor> gate_impl(const Tensor& scores, const OptTensor& mask, int64
   TORCH_CHECK_VALUE(K <= MAX_SLOTS && n <= MAX_SLOTS, "too many scores: ", scores.sizes());
   const MaskArg m = mask_of(mask, scores, n, K);
   const DevGuard guard(scores.device());
-  Tensor w = at::empty({n, k}, scores.options().dtype(at::kFloat));
-  Tensor labels = at::empty({n, k}, scores.options().dtype(at::kInt));
+  Tensor w = fresh({n, k}, at::kFloat, scores);
+  Tensor labels = fresh({n, k}, at::kInt, scores);
   std::vector<Tensor> res = {w, labels};
   Tensor stat;
   if (want_stat) {
-    stat = at::empty({n, 2}, scores.options().dtype(at::kFloat));
+    stat = fresh({n, 2}, at::kFloat, scores);
     res.push_back(stat);
   }
   check(tdc_topk_gate(code, scores.data_ptr(), scores.stride(0), m.p, m.rs, m.cs, n, (int)K, (int)k,
@@ -249,7 +255,7 @@ Tensor gate_bwd_impl(const OptTensor& scores, const OptTensor& mask, const Tenso
     m = mask_of(mask, *scores, n, K);
   }
   const DevGuard guard(w.device());
-  Tensor ds = at::empty({n, K}, w.options().dtype(dtype));
+  Tensor ds = fresh({n, K}, dtype, w);
   check(tdc_topk_gate_bwd(code, normalize ? nullptr : scores->data_ptr(),
                           normalize ? 0 : scores->stride(0), m.p, m.rs, m.cs, w.data_ptr<float>(),
                           labels.data_ptr<int32_t>(), normalize ? nullptr : stat->data_ptr<float>(),
@@ -271,13 +277,12 @@ std::vector<Tensor> group_plan(const Tensor& given, int64_t K) {
   TORCH_CHECK_VALUE(m <= MAX_SLOTS, "at most ", MAX_SLOTS, " labels, got ", m);
   const Tensor labels = given.contiguous();
   const DevGuard guard(labels.device());
-  const auto opt = labels.options().dtype(at::kInt);
-  Tensor offsets = at::empty({K + 1}, opt);
-  Tensor order = at::empty({m}, opt);
-  Tensor pos = at::empty(labels.sizes(), opt);
+  Tensor offsets = fresh({K + 1}, at::kInt, labels);
+  Tensor order = fresh({m}, at::kInt, labels);
+  Tensor pos = fresh(labels.sizes(), at::kInt, labels);
   const int64_t words = tdc_group_plan_work(m, (int)K);
   Tensor work;
-  if (words) work = at::empty({words}, opt);
+  if (words) work = fresh({words}, at::kInt, labels);
   check(tdc_group_plan(labels.scalar_type() == at::kLong, labels.data_ptr(), m, (int)K,
                        words ? work.data_ptr<int32_t>() : nullptr, order.data_ptr<int32_t>(),
                        pos.data_ptr<int32_t>(), offsets.data_ptr<int32_t>(), cur_stream()),
@@ -302,7 +307,7 @@ Tensor group_impl(const Tensor& x, const Tensor& offsets, const Tensor& pos) {
   TORCH_CHECK_VALUE(pos.size(0) == n, "the plan is of ", pos.size(0), " rows, x has ", n);
   TORCH_CHECK_VALUE(d <= MAX_COLUMNS, "at most ", MAX_COLUMNS, " columns, got ", d);
   const DevGuard guard(x.device());
-  Tensor out = at::empty({n * k, d}, x.options());
+  Tensor out = fresh({n * k, d}, x.scalar_type(), x);
   check(tdc_group_rows(code, x.data_ptr(), x.stride(0), n, (int)k, (int)d,
                        offsets.data_ptr<int32_t>(), (int)offsets.numel() - 1,
                        pos.data_ptr<int32_t>(), out.data_ptr(), cur_stream()),
@@ -320,7 +325,7 @@ Tensor combine_impl(const Tensor& y, const Tensor& offsets, const Tensor& pos, c
   bool w32;
   const void* wp = weights_of(w, y, pos.sizes(), "weights", w32);
   const DevGuard guard(y.device());
-  Tensor out = at::empty({n, d}, y.options());
+  Tensor out = fresh({n, d}, y.scalar_type(), y);
   check(tdc_combine_rows(code, y.data_ptr(), y.stride(0), n, (int)k, (int)d,
                          offsets.data_ptr<int32_t>(), (int)offsets.numel() - 1,
                          pos.data_ptr<int32_t>(), wp, w32, out.data_ptr(), cur_stream()),
@@ -349,11 +354,11 @@ std::vector<Tensor> combine_bwd_impl(const Tensor& dout, const OptTensor& y, con
   Tensor dy, dw;
   std::vector<Tensor> res;
   if (want_dy) {
-    dy = at::empty({n * k, d}, dout.options());
+    dy = fresh({n * k, d}, dout.scalar_type(), dout);
     res.push_back(dy);
   }
   if (want_dw) {
-    dw = at::empty(w->sizes(), w->options());
+    dw = fresh(w->sizes(), w->scalar_type(), *w);
     res.push_back(dw);
   }
   check(tdc_combine_rows_bwd(code, dout.data_ptr(), dout.stride(0),

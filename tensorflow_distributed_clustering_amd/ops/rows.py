@@ -42,18 +42,13 @@ def _ops():
     return _tdc
 
 
-def _on_gpu(**tensors) -> bool:
+def _on_gpu(x, a=None, b=None) -> bool:
     """Whether the kernels take the call.  Their bindings check its arguments themselves, with
     the errors of the checks below, which are the CPU path's: a request pays for one set."""
-    gpu = None
-    for name, t in tensors.items():
-        if t is None and gpu is not None:
-            continue
-        if not isinstance(t, torch.Tensor):
-            raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
-        if gpu is None:
-            gpu = t.is_cuda
-    return gpu
+    if (isinstance(x, torch.Tensor) and (a is None or isinstance(a, torch.Tensor))
+            and (b is None or isinstance(b, torch.Tensor))):
+        return x.is_cuda
+    raise TypeError(f"expected tensors, got {', '.join(type(t).__name__ for t in (x, a, b) if t is not None)}")
 
 
 def _check_rows(x, name: str):
@@ -98,7 +93,7 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
     [D] is fp32 or of the rows' type (None: ones).  The squares are summed in fp32: a row
     whose sum of squares passes 3.4e38 becomes zeros.  With ``eps`` = 0 a row of zeros
     becomes NaN."""
-    if not _on_gpu(x=x, weight=weight, residual=residual):
+    if not _on_gpu(x, weight, residual):
         _check_norm(x, weight, residual, eps)
         return ref.rms_norm(x, weight, residual, eps)
     out = _ops().rms_norm(x, weight, residual, eps)
@@ -143,7 +138,7 @@ def rms_norm_fp8(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
     """:func:`rms_norm` whose ``y`` is computed in fp64 and rounded once to
     :class:`Fp8Rows`, one exponent per 32 columns.  Returns the rows, or ``(rows, h)`` with a residual.  For
     serving: it has no gradient, and refuses inputs that ask for one."""
-    gpu = _on_gpu(x=x, weight=weight, residual=residual)
+    gpu = _on_gpu(x, weight, residual)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
         raise RuntimeError("rms_norm_fp8 has no gradient: call it under torch.no_grad()")
     if not gpu or x.dim() != 2:
@@ -169,7 +164,7 @@ def topk_gate(scores: torch.Tensor, k: int, mask: Optional[torch.Tensor] = None,
     never chosen, its score is not looked at and its gradient is zero.  Where fewer than k
     are left the last labels are -1 with weight 0, which :func:`group_plan` leaves out.  A
     NaN or +inf among the allowed scores makes the row's weights NaN."""
-    gpu = _on_gpu(scores=scores, mask=mask)
+    gpu = _on_gpu(scores, mask)
     k, normalize = int(k), bool(normalize)
     if mask is not None and mask.shape != scores.shape:
         try:
@@ -223,7 +218,7 @@ def group_plan(labels: torch.Tensor, n_clusters: int) -> RowGroups:
     sorted by cluster; rows of one cluster keep their order.  Labels outside
     [0, n_clusters) drop their slot.  The same labels give the same plan."""
     n_clusters = int(n_clusters)
-    if _on_gpu(labels=labels):
+    if _on_gpu(labels):
         return RowGroups(*_ops().group_plan(labels, n_clusters), n_clusters)
     if labels.dim() not in (1, 2) or labels.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"labels must be int32 or int64 [N] or [N, k], got {labels.dtype} "
@@ -247,7 +242,7 @@ def group_rows(x: torch.Tensor, groups: RowGroups) -> torch.Tensor:
     labels, zeros at the places from ``groups.offsets[-1]`` on.  The gradient sums a row's
     copies in fp32."""
     _check_groups(groups)
-    if _on_gpu(x=x):
+    if _on_gpu(x):
         return _ops().group_rows(x, groups.offsets, groups.pos)
     _check_rows(x, "x")
     if x.shape[0] != groups.n_rows or x.device != groups.pos.device:
@@ -262,7 +257,7 @@ def combine_rows(y: torch.Tensor, groups: RowGroups, weights: Optional[torch.Ten
     the shape of the plan's labels, fp32 or of the rows' type (None: ones).  Slots without a
     cluster add nothing, whatever ``y`` holds there; a row that has none left is zeros."""
     _check_groups(groups)
-    if _on_gpu(y=y, weights=weights):
+    if _on_gpu(y, weights):
         return _ops().combine_rows(y, groups.offsets, groups.pos, weights)
     _check_rows(y, "y")
     if y.shape[0] != groups.n_slots or y.device != groups.pos.device:
