@@ -120,7 +120,7 @@ template <typename In, int PER, bool LAST>
 __global__ __launch_bounds__(SORT_BLOCK) void sort_scatter_kernel(
     In in, int64_t m, int shift, int digits, int bits, const int* __restrict__ hist,
     const int* __restrict__ totals, int2* __restrict__ pairs, int* __restrict__ keys,
-    int* __restrict__ order, int* __restrict__ pos, int* __restrict__ offsets) {
+    int* __restrict__ order, int* __restrict__ pos, int* __restrict__ starts) {
   __shared__ int cnt[SORT_WAVES][MAX_DIGITS];
   __shared__ int s_total[MAX_DIGITS], s_before[MAX_DIGITS];
   __shared__ int s_wave[SORT_WAVES];
@@ -187,7 +187,7 @@ __global__ __launch_bounds__(SORT_BLOCK) void sort_scatter_kernel(
   for (int i = 0; i < own; ++i) {
     const int d = threadIdx.x * own + i;
     if (d < digits) {
-      if (offsets && chunk == 0) offsets[d] = at;
+      if (starts && chunk == 0) starts[d] = at;
       int next = at + s_before[d];
 #pragma unroll
       for (int q = 0; q < SORT_WAVES; ++q) {
@@ -237,15 +237,20 @@ __global__ __launch_bounds__(SORT_BLOCK) void sort_scatter_kernel(
 // where the second put what stood there: the slot's place is read through both (1M labels:
 // 18 us for the second pass and 11 here; 31 and 5 where that pass wrote pos[slot] itself, 4
 // bytes at a time all over).  offsets[c] is the first place whose key is c or more, looked
-// up by halving: as long for clusters that are all empty as for full ones.
-__global__ __launch_bounds__(SORT_BLOCK) void sort_finish_kernel(const int* __restrict__ keys,
-                                                                 const int* __restrict__ moved,
-                                                                 int m, int K, int* __restrict__ pos,
-                                                                 int* __restrict__ offsets) {
+// up by halving among the places of its upper digit (`starts`): as long for clusters that
+// are all empty as for full ones.
+__global__ __launch_bounds__(SORT_BLOCK) void sort_finish_kernel(
+    const int* __restrict__ keys, const int* __restrict__ moved, const int* __restrict__ starts,
+    int shift, int digits, int m, int K, int* __restrict__ pos, int* __restrict__ offsets) {
   const int64_t i = (int64_t)blockIdx.x * SORT_BLOCK + threadIdx.x;
   if (i < m) pos[i] = moved[min((unsigned)pos[i], (unsigned)m - 1)];
   if (i > K) return;
-  int lo = 0, hi = m;
+  int lo = 0, hi = 0;
+  if (m > 0) {
+    const int d = (int)(i >> shift);
+    lo = starts[d];
+    hi = d + 1 < digits ? starts[d + 1] : m;
+  }
   while (lo < hi) {
     const int mid = lo + (hi - lo) / 2;
     if (keys[mid] < i)
@@ -584,10 +589,10 @@ struct SortShape {
 
 using namespace tdc::rows;
 
-// int32 words of scratch of a plan (counts, totals and, with two passes, pairs, keys and moves).
+// int32 words of scratch of a plan (counts, totals and, with two passes, pairs, keys, moves and starts).
 int64_t tdc_group_plan_work(int64_t m, int K) {
   const SortShape s(m, K);
-  return s.count_words() + (s.high ? 4 * m : 0);
+  return s.count_words() + (s.high ? 4 * m + s.digits[1] : 0);
 }
 
 int tdc_group_plan(int wide_labels, const void* labels, int64_t m, int K, int* work, int* order,
@@ -599,6 +604,7 @@ int tdc_group_plan(int wide_labels, const void* labels, int64_t m, int K, int* w
   int2* pairs = s.high ? reinterpret_cast<int2*>(work + s.count_words()) : nullptr;
   int* keys = s.high ? work + s.count_words() + 2 * m : nullptr;
   int* moved = s.high ? keys + m : nullptr;
+  int* starts = s.high ? moved + m : nullptr;
   const dim3 grid((unsigned)s.chunks), block(SORT_BLOCK);
   auto pass = [&](auto in, auto last, auto per, int shift, int bits, int digits) {
     constexpr bool LAST = decltype(last)::value;
@@ -616,7 +622,8 @@ int tdc_group_plan(int wide_labels, const void* labels, int64_t m, int K, int* w
     }
     hipLaunchKernelGGL((sort_scatter_kernel<In, PER, LAST>), grid, block, 0, stream, in, m, shift,
                        digits, bits, hist, totals, pairs, LAST ? keys : nullptr, order,
-                       LAST && s.high ? moved : pos, s.high ? nullptr : offsets);
+                       LAST && s.high ? moved : pos,
+                       LAST ? (s.high ? starts : offsets) : nullptr);
     TDC_CHECK_LAUNCH();
     return 0;
   };
@@ -629,7 +636,8 @@ int tdc_group_plan(int wide_labels, const void* labels, int64_t m, int K, int* w
     }
     const int64_t items = std::max<int64_t>(m, K + 1);
     hipLaunchKernelGGL(sort_finish_kernel, dim3((unsigned)((items + SORT_BLOCK - 1) / SORT_BLOCK)),
-                       block, 0, stream, keys, moved, (int)m, K, pos, offsets);
+                       block, 0, stream, keys, moved, starts, s.low, s.digits[1], (int)m, K, pos,
+                       offsets);
     TDC_CHECK_LAUNCH();
     return 0;
   };
