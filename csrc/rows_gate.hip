@@ -146,7 +146,7 @@ __global__ __launch_bounds__(GATE_BLOCK) void gate_kernel(const T* __restrict__ 
                                                           float* __restrict__ stat) {
   constexpr int V = Vec<T>::N;
   constexpr unsigned INDEX = low_bits(L * R);  // the bits of a column
-  constexpr unsigned NONE = 0x007fffffu;      // the place of -inf: it and less is not chosen
+  constexpr unsigned NONE = 0x007fffffu;       // the place of -inf: it and less is not chosen
   __shared__ unsigned s_all[2][4];
   int turn = 0;
   const int lane = threadIdx.x % L;
@@ -182,9 +182,18 @@ __global__ __launch_bounds__(GATE_BLOCK) void gate_kernel(const T* __restrict__ 
     }
   }
   if (__any(nan)) {
+    // by what is allowed, not by the number so far: that of a NaN of all ones may be 0
 #pragma unroll
-    for (int i = 0; i < R; ++i)
-      if (v[i] != v[i] && num[i]) num[i] |= ~INDEX;
+    for (int i = 0; i < R / V; ++i) {
+      const int c = (i * L + lane) * V;
+      const unsigned in = MASKED ? ok[i].bits(mask, row, c, K) : 0u;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const bool there = MASKED ? (in >> j & 1) != 0 : c + j < K;
+        if (there && v[i * V + j] != v[i * V + j])
+          num[i * V + j] = ~INDEX | (INDEX - (unsigned)(c + j));
+      }
+    }
   }
   if (sizeof(T) == 4) lost = group_all<L>(lost, Any(), s_all, turn);
   unsigned limit = 0xffffffffu, before = 0, unsure = 0;
@@ -266,7 +275,8 @@ __device__ __forceinline__ void take_larger(unsigned& b, int& bi, unsigned ob, i
   }
 }
 
-// More clusters: a block per row, which is read again in every round (from the caches).  What is left is what comes after the last choice in the order.
+// More clusters: a block per row, which is read again in every round (from the caches).  What
+// is left is what comes after the last choice in the order.
 template <typename T>
 __global__ __launch_bounds__(GATE_BLOCK) void gate_wide_kernel(
     const T* __restrict__ scores, int64_t ld, Mask mask, int64_t n, int K, int k, bool normalize,

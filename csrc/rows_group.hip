@@ -276,11 +276,12 @@ __device__ __forceinline__ int kept_places(const int* offsets, int K, int64_t m)
 template <typename T, bool SHORT> __device__ __forceinline__ Raw16 take(const T* row, int c, int d) {
   return RowVec<T, SHORT ? TAIL_SHORT : TAIL_NONE>::fetch(row, c, d);
 }
-// f(STREAM): whether the sorted rows are stored past the caches: where they are as large as the last
-// level (256 MiB) they would only push out what the next kernel reads, and still be on their
-// way to memory then (131072 x 1024 bf16: grouped and the gradient summed 134 us past the
-// caches, 154 through them; grouped and read 422 us either way).  Smaller ones are kept for
-// their reader (64 MiB grouped and read: 104 us past the caches, 85 through them).
+
+// f(STREAM): whether the sorted rows are stored past the caches: where they are as large as
+// the last level (256 MiB) they would only push out what the next kernel reads, and still be
+// on their way to memory then (131072 x 1024 bf16: grouped and the gradient summed 134 us
+// past the caches, 154 through them; grouped and read 422 us either way).  Smaller ones are
+// kept for their reader (64 MiB grouped and read: 104 us past the caches, 85 through them).
 template <typename F> int with_stream(int64_t bytes, F&& f) {
   if (bytes >= (int64_t)256 << 20) return f(std::true_type());
   return f(std::false_type());

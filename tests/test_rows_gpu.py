@@ -201,6 +201,20 @@ def test_gate_nan_and_inf_that_are_allowed(gpu):
             assert lab.tolist() == [[1, 2], [1, 2]] and bool(w[0].isnan().all()) and bool(w[1, 0].isnan())
 
 
+@pytest.mark.parametrize("clusters", [64, 256, 1024, 8192, 9000])
+def test_gate_nan_of_all_ones(gpu, clusters):
+    s = normal(gpu, 1, 3, clusters)
+    s.view(torch.int32)[1, -1] = -1                  # memory filled with 0xff
+    s.view(torch.int32)[2, 5] = -1
+    m = torch.ones(3, clusters, dtype=torch.bool, device=gpu)
+    m[2, 5] = False
+    for mask, want in ((None, [clusters - 1, 5]), (m, [clusters - 1, -1])):
+        w, lab = tdc.topk_gate(s, 2, mask=mask)
+        assert int(lab[1, 0]) == want[0] and bool(w[1].isnan().all())
+        assert (int(lab[2, 0]) == 5) == (want[1] == 5) and bool(w[2].isnan().all()) == (want[1] == 5)
+        assert not bool(w[0].isnan().any())
+
+
 # ----------------------------------------------------------------- plan, group, combine
 @pytest.mark.parametrize("n,k,clusters", [(0, 2, 4), (1, 1, 1), (8, 2, 64), (4096, 1, 7), (4097, 1, 2047),
                                           (1500, 8, 256), (100, 1, 2048), (30000, 2, 65536),
