@@ -215,7 +215,7 @@ std::vector<Tensor> gate_impl(const Tensor& scores, const OptTensor& mask, int64
   const int code = code_of(scores.scalar_type(), "scores");
   TORCH_CHECK_VALUE(k >= 1 && k <= std::min<int64_t>(16, K), "k must be 1 to ",
                     std::min<int64_t>(16, K), ", got ", k);
-  TORCH_CHECK_VALUE(K <= MAX_SLOTS && n <= MAX_SLOTS, "too many scores: ", scores.sizes());
+  TORCH_CHECK_VALUE(K <= (1 << 30) && n <= MAX_SLOTS, "too many scores: ", scores.sizes());
   const MaskArg m = mask_of(mask, scores, n, K);
   const DevGuard guard(scores.device());
   Tensor w = fresh({n, k}, at::kFloat, scores);

@@ -141,7 +141,7 @@ def test_gradients_are_not_differentiable(gpu):
 
 # ----------------------------------------------------------------- gate
 @pytest.mark.parametrize("clusters,k", [(1, 1), (7, 7), (64, 2), (100, 16), (129, 3), (256, 8), (257, 6), (300, 9), (512, 7), (60, 8), (700, 16), (1500, 4),
-                                        (1000, 8), (1024, 16), (1025, 5), (4099, 16), (8192, 3), (8200, 5)])
+                                        (1000, 8), (1024, 16), (1025, 5), (4099, 16), (8192, 3), (8200, 5), (20001, 7)])
 @pytest.mark.parametrize("dtype", rc.DTYPES)
 def test_gate(gpu, clusters, k, dtype):
     n = 11
@@ -174,7 +174,7 @@ def test_gate(gpu, clusters, k, dtype):
             assert torch.equal(again[0], w) and torch.equal(again[1], lab)
 
 
-@pytest.mark.parametrize("clusters", [90, 256, 1000, 4096, 5000])
+@pytest.mark.parametrize("clusters", [90, 256, 1000, 4096, 9000, 30000])
 def test_gate_scores_that_differ_in_their_last_bits(gpu, clusters):
     g = torch.Generator().manual_seed(clusters)
     step = 2.0 ** -23
