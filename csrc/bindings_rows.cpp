@@ -403,6 +403,29 @@ variable_list once(variable_list grads, const variable_list& in, const variable_
   return grads;
 }
 
+// A gradient that is being captured may not go on to a node of the default stream, such as
+// the accumulator that a leaf keeps while an eager graph of it lives: the engine would have
+// that stream wait for the captured one, which ends the process.  Raises before it does.
+void check_capture() {
+  const at::hip::HIPStreamMasqueradingAsCUDA now = at::hip::getCurrentHIPStreamMasqueradingAsCUDA();
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(now.stream(), &status) != hipSuccess ||
+      status == hipStreamCaptureStatusNone)
+    return;
+  const auto node = torch::autograd::get_current_node();
+  if (!node) return;
+  const c10::Stream none =
+      at::hip::getDefaultHIPStreamMasqueradingAsCUDA(now.device_index()).unwrap();
+  for (const auto& edge : node->next_edges()) {
+    if (!edge.is_valid()) continue;
+    const auto stream = edge.function->stream();
+    TORCH_CHECK(!stream || stream->device_index() != none.device_index() || *stream != none,
+                "tdc: this gradient is being captured, but its input belongs to an autograd graph "
+                "made outside of the capture: capture the forward pass too, and drop other graphs "
+                "of the same leaves (or detach them) first");
+  }
+}
+
 OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; }
 
 struct RmsNorm : public Function<RmsNorm> {
@@ -418,6 +441,7 @@ struct RmsNorm : public Function<RmsNorm> {
     return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    check_capture();
     const auto saved = ctx->get_saved_variables();
     const bool residual = ctx->saved_data["residual"].toBool();
     const bool want_dw = ctx->saved_data["dw"].toBool();
@@ -453,6 +477,7 @@ struct TopkGate : public Function<TopkGate> {
     return {out[0], out[1]};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    check_capture();
     variable_list res(4);
     if (!grads[0].defined()) return res;
     const auto saved = ctx->get_saved_variables();
@@ -473,6 +498,7 @@ struct GroupRows : public Function<GroupRows> {
     return group_impl(x, offsets, pos);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    check_capture();
     const auto saved = ctx->get_saved_variables();
     variable_list res(3);
     res[0] = combine_impl(laid_out(grads[0]), saved[0], saved[1], std::nullopt);
@@ -488,6 +514,7 @@ struct CombineRows : public Function<CombineRows> {
     return combine_impl(y, offsets, pos, w);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    check_capture();
     const auto saved = ctx->get_saved_variables();
     const bool want_dy = ctx->saved_data["dy"].toBool();
     const std::vector<Tensor> g = combine_bwd_impl(laid_out(grads[0]), opt(saved[3]), saved[0],

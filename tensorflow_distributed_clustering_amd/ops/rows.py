@@ -14,7 +14,8 @@ tensors' device; CPU tensors run the same formulas in PyTorch (ops/reference.py)
 fp32, fp16 or bf16 [N, D] with contiguous columns and any row stride.  All but the fp8 norm
 are differentiable (once).  Nothing synchronises with the host and every buffer is a new
 tensor, so the calls can be captured into a HIP graph, the gradients too: capture forward
-and backward together, and keep no other live autograd graph of the same leaves.
+and backward together, with no other live autograd graph of the same leaves (a captured
+gradient that would go into one raises RuntimeError).
 """
 from __future__ import annotations
 

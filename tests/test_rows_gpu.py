@@ -458,3 +458,28 @@ def test_captured_forward_and_gradient(gpu, n, clusters):
         torch.cuda.synchronize()
         for a, b in zip(res, want):
             assert torch.equal(a, b)
+
+
+def test_capture_refuses_a_gradient_into_an_eager_graph(gpu):
+    x = normal(gpu, 1, 6, 40).requires_grad_()
+    groups = tdc.group_plan(torch.zeros(6, dtype=torch.int32, device=gpu), 2)
+    up = torch.ones(6, 40, device=gpu)
+    for op in (tdc.rms_norm, lambda t: tdc.group_rows(t, groups), lambda t: tdc.combine_rows(t, groups),
+               lambda t: tdc.topk_gate(t, 5)[0]):
+        op(x)
+        torch.cuda.synchronize()
+        eager = op(x)                                # its graph lives on
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match="outside of the capture"):
+            with torch.cuda.graph(graph):
+                y = op(x)
+                torch.autograd.grad(y, x, up[:, :y.shape[1]])
+        assert torch.isfinite(torch.autograd.grad(eager, x, up[:, :eager.shape[1]])[0]).all()
+        del eager, y
+        graph = torch.cuda.CUDAGraph()               # without it the same capture is fine
+        with torch.cuda.graph(graph):
+            y = op(x)
+            got, = torch.autograd.grad(y, x, up[:, :y.shape[1]])
+        graph.replay()
+        assert torch.equal(got, torch.autograd.grad(op(x), x, up[:, :y.shape[1]])[0])
+        del y, got
