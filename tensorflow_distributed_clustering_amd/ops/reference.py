@@ -248,7 +248,9 @@ def group_rows(x, offsets, order, pos):
 
 def combine_rows(y, offsets, pos, weights):
     p = pos.long().view(pos.shape[0], 1 if pos.dim() == 1 else pos.shape[1])
-    back = torch.where((p < offsets[-1])[..., None], y.float()[p], 0.0)
+    kept = (p < offsets[-1])[..., None]
+    back = torch.where(kept, y.float()[p], 0.0)
     if weights is not None:
-        back = back * weights.float().view(p.shape)[..., None]
+        # the weight too: 0 times an infinite one is not nothing
+        back = back * torch.where(kept, weights.float().view(p.shape)[..., None], 0.0)
     return back.sum(1).to(y.dtype)

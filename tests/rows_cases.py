@@ -110,6 +110,31 @@ def plan(labels, clusters):
     return t(offsets), t(order), t(pos).view(labels.shape)
 
 
+def check_dropped_weights(device, bad):
+    """Slots without a cluster add nothing to a row and get no gradient, whatever weight and
+    row they hold.  Every value is a small whole number: exact in any order."""
+    lab = torch.tensor([[0, -1], [5, 1], [-1, 7], [1, 0]], dtype=torch.int32, device=device)
+    drop = (lab < 0) | (lab >= 2)
+    w = torch.tensor([[2.0, 0.0], [0.0, 3.0], [0.0, 0.0], [1.0, -4.0]], device=device)
+    w = torch.where(drop, bad, w).requires_grad_()
+    groups = tdc.group_plan(lab, 2)
+    y = torch.arange(8.0, device=device)[:, None] + torch.tensor([0.0, 10.0, 20.0], device=device)
+    y[int(groups.offsets[-1]):] = bad
+    y.requires_grad_()
+    out = tdc.combine_rows(y, groups, w)
+    at = torch.where(drop, 0, groups.pos.long())
+    rows = y.detach()[at]                            # [4, 2, 3]; place 0 is kept
+    keep = torch.where(drop, 0.0, w.detach())[..., None]
+    assert torch.equal(out.detach(), (keep * rows).sum(1))
+    dout = torch.arange(12.0, device=device).view(4, 3)
+    dy, dw = torch.autograd.grad(out, (y, w), dout)
+    assert torch.equal(dw, torch.where(drop, 0.0, (rows * dout[:, None]).sum(2)))
+    want = torch.zeros(8, 3, device=device)
+    for r, j in (~drop).nonzero().tolist():
+        want[groups.pos[r, j].long()] = keep[r, j] * dout[r]
+    assert torch.equal(dy, want)
+
+
 # calls that are refused, on rows x [4, 8] and labels l [4] of either device
 REFUSALS = {
     "norm list": (lambda x, l: tdc.rms_norm([1.0]), TypeError),

@@ -134,6 +134,11 @@ def test_plan_group_combine(shape, clusters):
     assert torch.equal(dx, kept[:, None].expand(n, 6).float())
 
 
+@pytest.mark.parametrize("bad", [INF, -INF, float("nan")])
+def test_combine_never_looks_at_the_weight_of_a_dropped_slot(bad):
+    rc.check_dropped_weights(torch.device("cpu"), bad)
+
+
 # ----------------------------------------------------------------- refusals
 @pytest.mark.parametrize("name", rc.REFUSALS)
 def test_refusals(name):

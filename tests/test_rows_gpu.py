@@ -289,6 +289,11 @@ def test_group_and_combine(gpu, n, k, d, dtype):
             assert torch.equal(only, grads[1])
 
 
+@pytest.mark.parametrize("bad", [INF, -INF, float("nan")])
+def test_combine_never_looks_at_the_weight_of_a_dropped_slot(gpu, bad):
+    rc.check_dropped_weights(gpu, bad)
+
+
 # ----------------------------------------------------------------- refusals
 @pytest.mark.parametrize("name", rc.REFUSALS)
 def test_refusals(gpu, name):
