@@ -35,6 +35,9 @@ class ClusterPredictor:
         dev = torch.device(device) if device is not None else (
             torch.device("cuda", torch.cuda.current_device()) if torch.cuda.is_available()
             else torch.device("cpu"))
+        if dev.type == "cuda" and dev.index is None:
+            # the one that tensors made on "cuda" now get: "cuda" is unequal to their "cuda:0"
+            dev = torch.device("cuda", torch.cuda.current_device())
         self.k, self.d = int(c.shape[0]), int(c.shape[1])
         self.device = dev
         self.dtype = dtype

@@ -121,6 +121,18 @@ def test_predictor_reads_fp8_rows(gpu):
         assert torch.equal(parts, x[:n][order]) and torch.equal(groups.order.long(), order)
 
 
+def test_predictor_on_a_device_without_an_index(gpu):
+    x = normal(gpu, 1, 60, 40)
+    rows = tdc.rms_norm_fp8(x)
+    p = tdc.ClusterPredictor(x[:9], dtype="fp8", device="cuda")
+    q = tdc.ClusterPredictor(x[:9], dtype="fp8", device=gpu)
+    assert p.device == q.device
+    for got, want in zip(p.predict(rows, return_distance=True), q.predict(rows, return_distance=True)):
+        assert torch.equal(got, want)
+    parts, groups = p.partition(x)
+    assert parts.device == gpu and groups.offsets.device == gpu
+
+
 def test_gradients_are_not_differentiable(gpu):
     x, w = normal(gpu, 1, 6, 40).requires_grad_(), normal(gpu, 2, 40).requires_grad_()
     groups = tdc.group_plan(torch.zeros(6, dtype=torch.int32, device=gpu), 2)
