@@ -37,6 +37,7 @@ from ..config import ClusterConfig
 from ..data.stream import HostSource, ResidentSource, plan_chunk_rows, plan_resident_rows
 from ..ops import (NativeUpdate, acc_dtype_for, lloyd_fixed_extra, lloyd_layout, lloyd_row_extra,
                    make_lloyd_ops)
+from ..ops.rows import Fp8Rows
 from ..parallel.dist import Comm, join_counts, local_comm
 from ..utils import faults
 from ..utils.checkpoint import RunCheckpointer
@@ -961,11 +962,12 @@ class KMeans:
         return cache[key]
 
     def predict(self, x: torch.Tensor) -> torch.Tensor:
-        """Labels of new points against the fitted centroids (local, no collectives)."""
-        x = torch.as_tensor(x)
+        """Labels of new points against the fitted centroids (local, no collectives); of a
+        model with ``dtype="fp8"`` also those of :class:`Fp8Rows`."""
+        x = x if isinstance(x, Fp8Rows) else torch.as_tensor(x)
         return self.predictor(x.device).predict(x)
 
     def score(self, x: torch.Tensor) -> float:
         """Negative inertia of ``x`` (sklearn convention)."""
-        x = torch.as_tensor(x)
+        x = x if isinstance(x, Fp8Rows) else torch.as_tensor(x)
         return self.predictor(x.device).score(x)

@@ -25,6 +25,7 @@ import torch
 from ..config import ClusterConfig
 from ..data.stream import ResidentSource
 from ..ops import acc_dtype_for, make_lloyd_ops
+from ..ops.rows import Fp8Rows
 from ..parallel.dist import Comm, local_comm
 from ..utils import faults
 from ..utils.checkpoint import RunCheckpointer
@@ -218,9 +219,10 @@ class MiniBatchKMeans:
         return self
 
     def predict(self, x):
-        """Labels of new rows against the current centres."""
+        """Labels of new rows against the current centres; of a model with ``dtype="fp8"`` also
+        those of :class:`Fp8Rows`."""
         from ..serving import ClusterPredictor
-        x = torch.as_tensor(x)
+        x = x if isinstance(x, Fp8Rows) else torch.as_tensor(x)
         return ClusterPredictor(self.cluster_centers_, self.cfg.dtype, x.device,
                                 self.cfg.backend).predict(x)
 

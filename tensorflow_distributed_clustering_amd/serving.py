@@ -78,7 +78,9 @@ class ClusterPredictor:
         their squared distance to the chosen centroid (kernel arithmetic).  ``copy=False``
         returns the per-batch-size output buffers themselves (no extra kernel; valid until
         the next request of the same size).  ``x`` may be the :class:`Fp8Rows` of
-        ``rms_norm_fp8`` where the predictor is fp8: they are assigned as they are."""
+        ``rms_norm_fp8`` where the predictor is fp8: they are assigned as they are, into new
+        tensors whatever ``copy`` says, and not by a captured graph, which starts at rows
+        that are still to be quantised."""
         if isinstance(x, Fp8Rows):
             return self._predict_fp8(x, return_distance)
         x = torch.as_tensor(x)

@@ -176,3 +176,19 @@ def test_predictor_fp8_rows_and_partition():
     for k in range(9):
         at = groups.offsets[k:k + 2].tolist()
         assert torch.equal(parts[at[0]:at[1]], x[lab == k])
+
+
+def test_models_predict_fp8_rows():
+    g = gen(7)
+    x = torch.randn(200, 40, generator=g)
+    rows = tdc.rms_norm_fp8(x)
+    y = rows.dequantize()
+    km = tdc.KMeans(tdc.ClusterConfig(n_clusters=5, max_iter=3, dtype="fp8", seed=1)).fit(y)
+    assert torch.equal(km.predict(rows), km.predict(y))
+    assert km.score(rows) == km.score(y)
+    mb = tdc.MiniBatchKMeans(tdc.ClusterConfig(n_clusters=5, max_iter=3, dtype="fp8", batch_size=100, seed=1)).fit(y)
+    assert torch.equal(mb.predict(rows), mb.predict(y))
+    for model in (tdc.KMeans, tdc.MiniBatchKMeans):
+        other = model(tdc.ClusterConfig(n_clusters=5, max_iter=2, dtype="fp32", batch_size=100, seed=1)).fit(y)
+        with pytest.raises(ValueError, match="dtype='fp8'"):
+            other.predict(rows)

@@ -133,6 +133,18 @@ def test_predictor_on_a_device_without_an_index(gpu):
     assert parts.device == gpu and groups.offsets.device == gpu
 
 
+def test_models_predict_fp8_rows(gpu):
+    x = gaussian_blobs(3000, 200, 8, seed=3, dtype=torch.float32, device=gpu)
+    rows = tdc.rms_norm_fp8(x)
+    y = rows.dequantize(torch.bfloat16)
+    km = tdc.KMeans(tdc.ClusterConfig(n_clusters=8, max_iter=3, dtype="fp8", seed=1)).fit(y)
+    mb = tdc.MiniBatchKMeans(tdc.ClusterConfig(n_clusters=8, max_iter=3, dtype="fp8", batch_size=1000, seed=1)).fit(y)
+    for model, centers in ((km, km.result_.centers), (mb, mb.cluster_centers_)):
+        want = tdc.ClusterPredictor(centers, dtype="fp8", device=gpu).predict(rows)
+        assert torch.equal(model.predict(rows), want)
+    assert km.score(rows) < 0
+
+
 def test_gradients_are_not_differentiable(gpu):
     x, w = normal(gpu, 1, 6, 40).requires_grad_(), normal(gpu, 2, 40).requires_grad_()
     groups = tdc.group_plan(torch.zeros(6, dtype=torch.int32, device=gpu), 2)
