@@ -528,10 +528,23 @@ struct CombineRows : public Function<CombineRows> {
 
 bool no_graph() { return !at::GradMode::is_enabled(); }
 
+// There are no forward-mode formulas: an input with a tangent is refused, whether or not it
+// asks for a gradient, since the result would go on without one.
+void no_tangent(const Tensor& t, const char* what) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(/*level=*/0).defined(), "tdc: ", what,
+                              " has no forward-mode gradient");
+}
+void no_tangent(const OptTensor& t, const char* what) {
+  if (t.has_value()) no_tangent(*t, what);
+}
+
 std::vector<Tensor> rms_norm(const Tensor& x, const OptTensor& w, const OptTensor& r, double eps) {
   return norm_impl(x, w, r, eps, false, 0);
 }
 std::vector<Tensor> rms_norm_ad(const Tensor& x, const OptTensor& w, const OptTensor& r, double eps) {
+  no_tangent(x, "rms_norm");
+  no_tangent(w, "rms_norm");
+  no_tangent(r, "rms_norm");
   if (no_graph() || !(wants_grad(x) || wants_grad(w) || wants_grad(r))) return rms_norm(x, w, r, eps);
   return RmsNorm::apply(x, w, r, eps);
 }
@@ -541,6 +554,13 @@ std::vector<Tensor> rms_norm_fp8(const Tensor& x, const OptTensor& w, const OptT
   TORCH_CHECK(width > 0, "tdc.rms_norm_fp8: width");
   return norm_impl(x, w, r, eps, false, width);
 }
+std::vector<Tensor> rms_norm_fp8_ad(const Tensor& x, const OptTensor& w, const OptTensor& r,
+                                    double eps, int64_t width) {
+  no_tangent(x, "rms_norm_fp8");
+  no_tangent(w, "rms_norm_fp8");
+  no_tangent(r, "rms_norm_fp8");
+  return rms_norm_fp8(x, w, r, eps, width);
+}
 
 std::tuple<Tensor, Tensor> topk_gate(const Tensor& scores, const OptTensor& mask, int64_t k,
                                      bool normalize) {
@@ -549,6 +569,7 @@ std::tuple<Tensor, Tensor> topk_gate(const Tensor& scores, const OptTensor& mask
 }
 std::tuple<Tensor, Tensor> topk_gate_ad(const Tensor& scores, const OptTensor& mask, int64_t k,
                                         bool normalize) {
+  no_tangent(scores, "topk_gate");
   if (no_graph() || !wants_grad(scores)) return topk_gate(scores, mask, k, normalize);
   const variable_list out = TopkGate::apply(scores, mask, k, normalize);
   return {out[0], out[1]};
@@ -558,6 +579,7 @@ Tensor group_rows(const Tensor& x, const Tensor& offsets, const Tensor& pos) {
   return group_impl(x, offsets, pos);
 }
 Tensor group_rows_ad(const Tensor& x, const Tensor& offsets, const Tensor& pos) {
+  no_tangent(x, "group_rows");
   if (no_graph() || !wants_grad(x)) return group_impl(x, offsets, pos);
   return GroupRows::apply(x, offsets, pos);
 }
@@ -566,6 +588,8 @@ Tensor combine_rows(const Tensor& y, const Tensor& offsets, const Tensor& pos, c
   return combine_impl(y, offsets, pos, w);
 }
 Tensor combine_rows_ad(const Tensor& y, const Tensor& offsets, const Tensor& pos, const OptTensor& w) {
+  no_tangent(y, "combine_rows");
+  no_tangent(w, "combine_rows");
   if (no_graph() || !(wants_grad(y) || wants_grad(w))) return combine_impl(y, offsets, pos, w);
   return CombineRows::apply(y, offsets, pos, w);
 }
@@ -594,6 +618,7 @@ TORCH_LIBRARY_IMPL(tdc, CUDA, m) {
 
 TORCH_LIBRARY_IMPL(tdc, AutogradCUDA, m) {
   m.impl("rms_norm", &rms_norm_ad);
+  m.impl("rms_norm_fp8", &rms_norm_fp8_ad);
   m.impl("topk_gate", &topk_gate_ad);
   m.impl("group_rows", &group_rows_ad);
   m.impl("combine_rows", &combine_rows_ad);

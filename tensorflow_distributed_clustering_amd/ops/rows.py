@@ -12,10 +12,11 @@ What a model does to its rows (tokens, embeddings) around their assignment to cl
 On the GPU every one runs its HIP kernel (csrc/rows_*.hip), on the current stream of its
 tensors' device; CPU tensors run the same formulas in PyTorch (ops/reference.py).  Rows are
 fp32, fp16 or bf16 [N, D] with contiguous columns and any row stride.  All but the fp8 norm
-are differentiable (once).  Nothing synchronises with the host and every buffer is a new
-tensor, so the calls can be captured into a HIP graph, the gradients too: capture forward
-and backward together, with no other live autograd graph of the same leaves (a captured
-gradient that would go into one raises RuntimeError).
+are differentiable (once, and backward: a GPU tensor with a forward-mode tangent raises
+NotImplementedError).  Nothing synchronises with the host and every buffer is a new tensor,
+so the calls can be captured into a HIP graph, the gradients too: capture forward and
+backward together, with no other live autograd graph of the same leaves (a captured gradient
+that would go into one raises RuntimeError).
 """
 from __future__ import annotations
 
@@ -23,6 +24,7 @@ import math
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from .. import _native
 from . import fp8_dim, reference as ref
@@ -142,6 +144,8 @@ def rms_norm_fp8(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
     gpu = _on_gpu(x, weight, residual)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
         raise RuntimeError("rms_norm_fp8 has no gradient: call it under torch.no_grad()")
+    if not gpu and any(t is not None and unpack_dual(t).tangent is not None for t in (x, weight, residual)):
+        raise NotImplementedError("rms_norm_fp8 has no forward-mode gradient")
     if not gpu or x.dim() != 2:
         _check_norm(x, weight, residual, eps)
     d = x.shape[1]

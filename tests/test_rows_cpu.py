@@ -2,6 +2,7 @@
 differences, refusals, the predictor's fp8 rows and partition."""
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 
 import tensorflow_distributed_clustering_amd as tdc
 from tensorflow_distributed_clustering_amd.ops import rows as R
@@ -192,3 +193,24 @@ def test_models_predict_fp8_rows():
         other = model(tdc.ClusterConfig(n_clusters=5, max_iter=2, dtype="fp32", batch_size=100, seed=1)).fit(y)
         with pytest.raises(ValueError, match="dtype='fp8'"):
             other.predict(rows)
+
+
+def test_fp8_norm_refuses_forward_mode():
+    x, w = torch.randn(4, 40, generator=gen(9)), torch.ones(40)
+    with torch.no_grad(), fwd.dual_level():
+        for args in ((fwd.make_dual(x, x), w, None), (x, fwd.make_dual(w, w), None), (x, w, fwd.make_dual(x, x))):
+            with pytest.raises(RuntimeError, match="gradient"):
+                tdc.rms_norm_fp8(*args)
+        assert tdc.rms_norm_fp8(x, w).shape == (4, 40)
+
+
+def test_forward_mode():
+    """The CPU path has the tangents that the GPU refuses: against differences of the formula."""
+    g = gen(10)
+    x, w, t = torch.randn(4, 40, generator=g), torch.randn(40, generator=g), torch.randn(4, 40, generator=g)
+    with fwd.dual_level():
+        y = fwd.unpack_dual(tdc.rms_norm(fwd.make_dual(x, t), w, eps=1e-5)).tangent
+    step = 1e-6
+    up, down = (rc.norm(x.double() + s * t.double(), w, 1e-5)[1] for s in (step, -step))
+    # values of order 10: fp32 arithmetic of a few roundings, differences of order step^2
+    assert torch.allclose(y.double(), (up - down) / (2 * step), rtol=1e-5, atol=1e-5)
