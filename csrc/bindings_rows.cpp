@@ -140,8 +140,22 @@ std::vector<Tensor> norm_impl(const Tensor& x, const OptTensor& w, const OptTens
   return res;
 }
 
-std::vector<Tensor> norm_bwd_impl(const Tensor& h, const OptTensor& w, const Tensor& rstd,
-                                  const Tensor& dy, const OptTensor& dh, bool want_dw) {
+std::vector<Tensor> rms_norm(const Tensor& x, const OptTensor& w, const OptTensor& r, double eps) {
+  return norm_impl(x, w, r, eps, false, 0);
+}
+// with what the gradient needs: y[, h], rstd
+std::vector<Tensor> rms_norm_train(const Tensor& x, const OptTensor& w, const OptTensor& r,
+                                   double eps) {
+  return norm_impl(x, w, r, eps, true, 0);
+}
+std::vector<Tensor> rms_norm_fp8(const Tensor& x, const OptTensor& w, const OptTensor& r, double eps,
+                                 int64_t width) {
+  TORCH_CHECK(width > 0, "tdc.rms_norm_fp8: width");
+  return norm_impl(x, w, r, eps, false, width);
+}
+
+std::vector<Tensor> rms_norm_bwd(const Tensor& h, const OptTensor& w, const Tensor& rstd,
+                                 const Tensor& dy, const OptTensor& dh, bool want_dw) {
   check_rows(h, "h");
   check_like(dy, h, "dy");
   if (has(dh)) check_like(*dh, h, "dh");
@@ -233,8 +247,19 @@ std::vector<Tensor> gate_impl(const Tensor& scores, const OptTensor& mask, int64
   return res;
 }
 
+std::tuple<Tensor, Tensor> topk_gate(const Tensor& scores, const OptTensor& mask, int64_t k,
+                                     bool normalize) {
+  const std::vector<Tensor> out = gate_impl(scores, mask, k, normalize, false);
+  return {out[0], out[1]};
+}
+// with what the gradient over all clusters needs: w, labels[, stat]
+std::vector<Tensor> topk_gate_train(const Tensor& scores, const OptTensor& mask, int64_t k,
+                                    bool normalize) {
+  return gate_impl(scores, mask, k, normalize, !normalize);
+}
+
 // scores, mask, stat: given without `normalize` only.
-Tensor gate_bwd_impl(const OptTensor& scores, const OptTensor& mask, const Tensor& w,
+Tensor topk_gate_bwd(const OptTensor& scores, const OptTensor& mask, const Tensor& w,
                      const Tensor& labels, const OptTensor& stat, const Tensor& dw, int64_t K,
                      at::ScalarType dtype) {
   TORCH_CHECK(w.is_cuda() && w.dim() == 2 && w.scalar_type() == at::kFloat && w.is_contiguous(),
@@ -300,7 +325,7 @@ int64_t slots_of(const Tensor& offsets, const Tensor& pos, const Tensor& like) {
   return pos.dim() == 1 ? 1 : pos.size(1);
 }
 
-Tensor group_impl(const Tensor& x, const Tensor& offsets, const Tensor& pos) {
+Tensor group_rows(const Tensor& x, const Tensor& offsets, const Tensor& pos) {
   check_rows(x, "x");
   const int64_t n = x.size(0), d = x.size(1), k = slots_of(offsets, pos, x);
   const int code = code_of(x.scalar_type(), "x");
@@ -315,7 +340,7 @@ Tensor group_impl(const Tensor& x, const Tensor& offsets, const Tensor& pos) {
   return out;
 }
 
-Tensor combine_impl(const Tensor& y, const Tensor& offsets, const Tensor& pos, const OptTensor& w) {
+Tensor combine_rows(const Tensor& y, const Tensor& offsets, const Tensor& pos, const OptTensor& w) {
   check_rows(y, "y");
   const int64_t n = pos.size(0), d = y.size(1), k = slots_of(offsets, pos, y);
   const int code = code_of(y.scalar_type(), "y");
@@ -334,7 +359,7 @@ Tensor combine_impl(const Tensor& y, const Tensor& offsets, const Tensor& pos, c
 }
 
 // y: given where the weights' gradient is wanted.
-std::vector<Tensor> combine_bwd_impl(const Tensor& dout, const OptTensor& y, const Tensor& offsets,
+std::vector<Tensor> combine_rows_bwd(const Tensor& dout, const OptTensor& y, const Tensor& offsets,
                                      const Tensor& pos, const OptTensor& w, bool want_dy) {
   check_rows(dout, "dout");
   const int64_t n = dout.size(0), d = dout.size(1), k = slots_of(offsets, pos, dout);
@@ -374,6 +399,17 @@ std::vector<Tensor> combine_bwd_impl(const Tensor& dout, const OptTensor& y, con
 using torch::autograd::AutogradContext;
 using torch::autograd::Function;
 using torch::autograd::variable_list;
+
+// The operator tdc::NAME below autograd, with the signature of its kernel.  Not the kernel
+// itself: what stands between the two (dispatch modes, tracing) sees the call as it sees
+// PyTorch's own (0.5 us of a call).
+#define TDC_BELOW_AUTOGRAD(NAME, ...)                                                     \
+  [&] {                                                                                   \
+    static const auto op =                                                                \
+        c10::Dispatcher::singleton().findSchemaOrThrow("tdc::" #NAME, "").typed<decltype(NAME)>(); \
+    const at::AutoDispatchBelowADInplaceOrView below;                                     \
+    return op.call(__VA_ARGS__);                                                          \
+  }()
 
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
 bool wants_grad(const OptTensor& t) { return has(t) && t->requires_grad(); }
@@ -431,7 +467,7 @@ OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullop
 struct RmsNorm : public Function<RmsNorm> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const OptTensor& w,
                                const OptTensor& r, double eps) {
-    std::vector<Tensor> out = norm_impl(x, w, r, eps, true, 0);
+    std::vector<Tensor> out = TDC_BELOW_AUTOGRAD(rms_norm_train, x, w, r, eps);
     Tensor rstd = out.back();
     out.pop_back();
     ctx->set_materialize_grads(false);
@@ -451,7 +487,8 @@ struct RmsNorm : public Function<RmsNorm> {
       res[0] = dh;
     } else {
       const std::vector<Tensor> g =
-          norm_bwd_impl(saved[0], opt(saved[1]), saved[2], laid_out(grads[0]), opt(dh), want_dw);
+          TDC_BELOW_AUTOGRAD(rms_norm_bwd, saved[0], opt(saved[1]), saved[2], laid_out(grads[0]),
+                             opt(dh), want_dw);
       res[0] = g[0];
       if (want_dw) res[1] = g[1];
     }
@@ -463,7 +500,7 @@ struct RmsNorm : public Function<RmsNorm> {
 struct TopkGate : public Function<TopkGate> {
   static variable_list forward(AutogradContext* ctx, const Tensor& scores, const OptTensor& mask,
                                int64_t k, bool normalize) {
-    std::vector<Tensor> out = gate_impl(scores, mask, k, normalize, !normalize);
+    std::vector<Tensor> out = TDC_BELOW_AUTOGRAD(topk_gate_train, scores, mask, k, normalize);
     ctx->set_materialize_grads(false);
     ctx->mark_non_differentiable({out[1]});
     // the weights over the chosen say all about their gradient; those over every cluster
@@ -482,11 +519,12 @@ struct TopkGate : public Function<TopkGate> {
     if (!grads[0].defined()) return res;
     const auto saved = ctx->get_saved_variables();
     const bool normalize = saved.size() == 2;
-    res[0] = gate_bwd_impl(normalize ? std::nullopt : opt(saved[2]),
-                           normalize ? std::nullopt : opt(saved[4]), saved[0], saved[1],
-                           normalize ? std::nullopt : opt(saved[3]), grads[0].contiguous(),
-                           ctx->saved_data["clusters"].toInt(),
-                           (at::ScalarType)ctx->saved_data["dtype"].toInt());
+    const OptTensor none;
+    res[0] = TDC_BELOW_AUTOGRAD(topk_gate_bwd, normalize ? none : opt(saved[2]),
+                                normalize ? none : opt(saved[4]), saved[0], saved[1],
+                                normalize ? none : opt(saved[3]), grads[0].contiguous(),
+                                ctx->saved_data["clusters"].toInt(),
+                                (at::ScalarType)ctx->saved_data["dtype"].toInt());
     return once(res, grads, saved);
   }
 };
@@ -495,13 +533,13 @@ struct GroupRows : public Function<GroupRows> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& offsets,
                         const Tensor& pos) {
     ctx->save_for_backward({offsets, pos});
-    return group_impl(x, offsets, pos);
+    return TDC_BELOW_AUTOGRAD(group_rows, x, offsets, pos);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     check_capture();
     const auto saved = ctx->get_saved_variables();
     variable_list res(3);
-    res[0] = combine_impl(laid_out(grads[0]), saved[0], saved[1], std::nullopt);
+    res[0] = TDC_BELOW_AUTOGRAD(combine_rows, laid_out(grads[0]), saved[0], saved[1], OptTensor());
     return once(res, grads, saved);
   }
 };
@@ -511,14 +549,15 @@ struct CombineRows : public Function<CombineRows> {
                         const Tensor& pos, const OptTensor& w) {
     ctx->save_for_backward({offsets, pos, has(w) ? *w : Tensor(), wants_grad(w) ? y : Tensor()});
     ctx->saved_data["dy"] = wants_grad(y);
-    return combine_impl(y, offsets, pos, w);
+    return TDC_BELOW_AUTOGRAD(combine_rows, y, offsets, pos, w);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     check_capture();
     const auto saved = ctx->get_saved_variables();
     const bool want_dy = ctx->saved_data["dy"].toBool();
-    const std::vector<Tensor> g = combine_bwd_impl(laid_out(grads[0]), opt(saved[3]), saved[0],
-                                                   saved[1], opt(saved[2]), want_dy);
+    const std::vector<Tensor> g =
+        TDC_BELOW_AUTOGRAD(combine_rows_bwd, laid_out(grads[0]), opt(saved[3]), saved[0], saved[1],
+                           opt(saved[2]), want_dy);
     variable_list res(4);
     if (want_dy) res[0] = g[0];
     if (saved[3].defined()) res[3] = g.back();
@@ -538,59 +577,43 @@ void no_tangent(const OptTensor& t, const char* what) {
   if (t.has_value()) no_tangent(*t, what);
 }
 
-std::vector<Tensor> rms_norm(const Tensor& x, const OptTensor& w, const OptTensor& r, double eps) {
-  return norm_impl(x, w, r, eps, false, 0);
-}
 std::vector<Tensor> rms_norm_ad(const Tensor& x, const OptTensor& w, const OptTensor& r, double eps) {
   no_tangent(x, "rms_norm");
   no_tangent(w, "rms_norm");
   no_tangent(r, "rms_norm");
-  if (no_graph() || !(wants_grad(x) || wants_grad(w) || wants_grad(r))) return rms_norm(x, w, r, eps);
+  if (no_graph() || !(wants_grad(x) || wants_grad(w) || wants_grad(r)))
+    return TDC_BELOW_AUTOGRAD(rms_norm, x, w, r, eps);
   return RmsNorm::apply(x, w, r, eps);
 }
 
-std::vector<Tensor> rms_norm_fp8(const Tensor& x, const OptTensor& w, const OptTensor& r, double eps,
-                                 int64_t width) {
-  TORCH_CHECK(width > 0, "tdc.rms_norm_fp8: width");
-  return norm_impl(x, w, r, eps, false, width);
-}
 std::vector<Tensor> rms_norm_fp8_ad(const Tensor& x, const OptTensor& w, const OptTensor& r,
                                     double eps, int64_t width) {
   no_tangent(x, "rms_norm_fp8");
   no_tangent(w, "rms_norm_fp8");
   no_tangent(r, "rms_norm_fp8");
-  return rms_norm_fp8(x, w, r, eps, width);
+  return TDC_BELOW_AUTOGRAD(rms_norm_fp8, x, w, r, eps, width);
 }
 
-std::tuple<Tensor, Tensor> topk_gate(const Tensor& scores, const OptTensor& mask, int64_t k,
-                                     bool normalize) {
-  const std::vector<Tensor> out = gate_impl(scores, mask, k, normalize, false);
-  return {out[0], out[1]};
-}
 std::tuple<Tensor, Tensor> topk_gate_ad(const Tensor& scores, const OptTensor& mask, int64_t k,
                                         bool normalize) {
   no_tangent(scores, "topk_gate");
-  if (no_graph() || !wants_grad(scores)) return topk_gate(scores, mask, k, normalize);
+  if (no_graph() || !wants_grad(scores))
+    return TDC_BELOW_AUTOGRAD(topk_gate, scores, mask, k, normalize);
   const variable_list out = TopkGate::apply(scores, mask, k, normalize);
   return {out[0], out[1]};
 }
 
-Tensor group_rows(const Tensor& x, const Tensor& offsets, const Tensor& pos) {
-  return group_impl(x, offsets, pos);
-}
 Tensor group_rows_ad(const Tensor& x, const Tensor& offsets, const Tensor& pos) {
   no_tangent(x, "group_rows");
-  if (no_graph() || !wants_grad(x)) return group_impl(x, offsets, pos);
+  if (no_graph() || !wants_grad(x)) return TDC_BELOW_AUTOGRAD(group_rows, x, offsets, pos);
   return GroupRows::apply(x, offsets, pos);
 }
 
-Tensor combine_rows(const Tensor& y, const Tensor& offsets, const Tensor& pos, const OptTensor& w) {
-  return combine_impl(y, offsets, pos, w);
-}
 Tensor combine_rows_ad(const Tensor& y, const Tensor& offsets, const Tensor& pos, const OptTensor& w) {
   no_tangent(y, "combine_rows");
   no_tangent(w, "combine_rows");
-  if (no_graph() || !(wants_grad(y) || wants_grad(w))) return combine_impl(y, offsets, pos, w);
+  if (no_graph() || !(wants_grad(y) || wants_grad(w)))
+    return TDC_BELOW_AUTOGRAD(combine_rows, y, offsets, pos, w);
   return CombineRows::apply(y, offsets, pos, w);
 }
 
@@ -604,6 +627,14 @@ TORCH_LIBRARY_FRAGMENT(tdc, m) {
   m.def("group_plan(Tensor labels, int K) -> Tensor[]");
   m.def("group_rows(Tensor x, Tensor offsets, Tensor pos) -> Tensor");
   m.def("combine_rows(Tensor y, Tensor offsets, Tensor pos, Tensor? w) -> Tensor");
+  // the two halves of the autograd nodes
+  m.def("rms_norm_train(Tensor x, Tensor? w, Tensor? r, float eps) -> Tensor[]");
+  m.def("rms_norm_bwd(Tensor h, Tensor? w, Tensor rstd, Tensor dy, Tensor? dh, bool want_dw) -> Tensor[]");
+  m.def("topk_gate_train(Tensor scores, Tensor? mask, int k, bool normalize) -> Tensor[]");
+  m.def("topk_gate_bwd(Tensor? scores, Tensor? mask, Tensor w, Tensor labels, Tensor? stat, "
+        "Tensor dw, int K, ScalarType dtype) -> Tensor");
+  m.def("combine_rows_bwd(Tensor dout, Tensor? y, Tensor offsets, Tensor pos, Tensor? w, "
+        "bool want_dy) -> Tensor[]");
 }
 
 TORCH_LIBRARY_IMPL(tdc, CUDA, m) {
@@ -614,6 +645,11 @@ TORCH_LIBRARY_IMPL(tdc, CUDA, m) {
   m.impl("group_plan", &group_plan);
   m.impl("group_rows", &group_rows);
   m.impl("combine_rows", &combine_rows);
+  m.impl("rms_norm_train", &rms_norm_train);
+  m.impl("rms_norm_bwd", &rms_norm_bwd);
+  m.impl("topk_gate_train", &topk_gate_train);
+  m.impl("topk_gate_bwd", &topk_gate_bwd);
+  m.impl("combine_rows_bwd", &combine_rows_bwd);
 }
 
 TORCH_LIBRARY_IMPL(tdc, AutogradCUDA, m) {

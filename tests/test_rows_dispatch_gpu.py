@@ -1,7 +1,10 @@
-"""Row operators under PyTorch's own machinery on the GPU: forward-mode gradients."""
+"""Row operators under PyTorch's own machinery on the GPU: forward-mode gradients, dispatch
+modes, tracing."""
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd
+from torch.fx.experimental.proxy_tensor import make_fx
+from torch.utils._python_dispatch import TorchDispatchMode
 
 import tensorflow_distributed_clustering_amd as tdc
 
@@ -36,6 +39,13 @@ def tuple_of(out):
     return out if isinstance(out, tuple) else (out,)
 
 
+def with_grads(gpu, call, leaves):
+    """Outputs and all gradients, as tensors without a graph."""
+    leaves = [t.detach().requires_grad_() for t in leaves]
+    outs = tuple_of(call(gpu, *leaves))
+    return tuple(o.detach() for o in outs) + torch.autograd.grad(outs, leaves, [o.detach() * 0.5 for o in outs])
+
+
 @pytest.mark.parametrize("name", CALLS)
 def test_forward_mode_is_refused(gpu, name):
     call, shapes = CALLS[name]
@@ -64,3 +74,45 @@ def test_fp8_norm_refuses_forward_mode(gpu):
         for args in ((fwd.make_dual(x, x), w, None), (x, fwd.make_dual(w, w), None), (x, w, fwd.make_dual(x, x))):
             with pytest.raises(RuntimeError, match="gradient"):
                 tdc.rms_norm_fp8(*args)
+
+
+class Seen(TorchDispatchMode):
+    """The operators of the package that pass, and what they return."""
+
+    def __init__(self):
+        super().__init__()
+        self.names, self.outs = [], {}
+
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        out = func(*args, **(kwargs or {}))
+        if func.namespace == "tdc":
+            name = func.name().split("::")[1]
+            self.names.append(name)
+            self.outs[name] = out
+        return out
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_dispatch_modes_see_the_calls(gpu, name):
+    call, _ = CALLS[name]
+    args = inputs(gpu, name)
+    want, grads = tuple_of(call(gpu, *args)), with_grads(gpu, call, args)
+    for run, result in ((lambda: tuple_of(call(gpu, *args)), want), (lambda: with_grads(gpu, call, args), grads)):
+        with Seen() as seen:
+            got = run()
+        assert all(torch.equal(a, b) for a, b in zip(got, result)) and len(got) == len(result)
+        stem = {"norm": "rms_norm", "gate": "topk_gate", "group": "group_rows", "combine": "combine_rows"}[name.split()[0]]
+        assert any(n.startswith(stem) for n in seen.names), seen.names
+    # the gradient too: one call more than its forward pass, the plan aside
+    assert len([n for n in seen.names if n != "group_plan"]) == 2, seen.names
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_traced_on_one_input_and_run_on_another(gpu, name):
+    call, _ = CALLS[name]
+    args, other = inputs(gpu, name), inputs(gpu, name, seed=10)
+    for f in (lambda *a: tuple_of(call(gpu, *a)), lambda *a: with_grads(gpu, call, a)):
+        graph = make_fx(f, tracing_mode="real")(*args)
+        for given in (args, other):
+            for a, b in zip(graph(*given), f(*given)):
+                assert torch.equal(a, b)
