@@ -22,6 +22,7 @@ namespace {
 
 using at::Tensor;
 using OptTensor = std::optional<Tensor>;
+using c10::SymInt;
 using DevGuard = at::hip::HIPGuardMasqueradingAsCUDA;
 
 hipStream_t cur_stream() { return at::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream(); }
@@ -52,40 +53,41 @@ Tensor fresh(at::IntArrayRef sizes, at::ScalarType t, const Tensor& like) {
 
 bool has(const OptTensor& t) { return t.has_value() && t->defined(); }
 
-// Arguments that a caller gets wrong raise ValueError, as the checks of the CPU path do.
+// Arguments that a caller gets wrong raise ValueError, as the checks of the CPU path do.  The
+// checks are those of the shape functions too, where sizes may be symbols.
 void check_rows(const Tensor& x, const char* name) {
-  TORCH_CHECK_VALUE(x.dim() == 2, name, " must be rows [N, D], got ", x.sizes());
-  TORCH_CHECK_VALUE(x.size(1) >= 1, name, " has no columns");
-  TORCH_CHECK_VALUE(x.stride(1) == 1 || x.size(1) == 1, name,
-                    " must have contiguous columns, got strides ", x.strides());
+  TORCH_CHECK_VALUE(x.dim() == 2, name, " must be rows [N, D], got ", x.sym_sizes());
+  TORCH_CHECK_VALUE(x.sym_size(1) >= 1, name, " has no columns");
+  TORCH_CHECK_VALUE(x.sym_stride(1) == 1 || x.sym_size(1) == 1, name,
+                    " must have contiguous columns, got strides ", x.sym_strides());
 }
 
 void check_like(const Tensor& t, const Tensor& x, const char* name) {
   check_rows(t, name);
   TORCH_CHECK_VALUE(t.device() == x.device() && t.scalar_type() == x.scalar_type() &&
-                        t.sizes() == x.sizes(),
+                        t.sym_sizes() == x.sym_sizes(),
                     name, " must have the shape, type and device of the rows");
 }
 
 // Weights of shape `sizes`: null, fp32 (w32) or the rows' type.
-const void* weights_of(const OptTensor& w, const Tensor& x, at::IntArrayRef sizes, const char* name,
-                       bool& w32) {
-  w32 = true;
-  if (!has(w)) return nullptr;
-  TORCH_CHECK_VALUE(w->sizes() == sizes && w->is_contiguous(), name, " must be contiguous ", sizes,
-                    ", got ", w->sizes());
+void check_weights(const OptTensor& w, const Tensor& x, c10::SymIntArrayRef sizes, const char* name) {
+  if (!has(w)) return;
+  TORCH_CHECK_VALUE(w->sym_sizes() == sizes && w->is_contiguous(), name, " must be contiguous ",
+                    sizes, ", got ", w->sym_sizes());
   TORCH_CHECK_VALUE(w->device() == x.device(), name, " is on ", w->device(), ", the rows on ",
                     x.device());
-  w32 = w->scalar_type() == at::kFloat;
-  TORCH_CHECK_VALUE(w32 || w->scalar_type() == x.scalar_type(), name,
+  TORCH_CHECK_VALUE(w->scalar_type() == at::kFloat || w->scalar_type() == x.scalar_type(), name,
                     " must be fp32 or of the rows' type, got ", w->scalar_type());
-  return w->data_ptr();
+}
+const void* weights_of(const OptTensor& w, bool& w32) {
+  w32 = !has(w) || w->scalar_type() == at::kFloat;
+  return has(w) ? w->data_ptr() : nullptr;
 }
 
-void check_index(const Tensor& t, const Tensor& x, int64_t n, const char* name) {
+void check_index(const Tensor& t, const Tensor& x, const SymInt& n, const char* name) {
   TORCH_CHECK_VALUE(t.device() == x.device(), "the plan is on ", t.device(), ", the rows on ",
                     x.device());
-  TORCH_CHECK_VALUE(t.scalar_type() == at::kInt && t.is_contiguous() && t.numel() == n, "tdc: ", name,
+  TORCH_CHECK_VALUE(t.scalar_type() == at::kInt && t.is_contiguous() && t.sym_numel() == n, "tdc: ", name,
                     " must be int32 [", n, "]");
 }
 
@@ -98,18 +100,25 @@ int num_cus(const Tensor& t) {
 }
 
 // ------------------------------------------------------------------ norm
-std::vector<Tensor> norm_impl(const Tensor& x, const OptTensor& w, const OptTensor& r, double eps,
-                              bool want_rstd, int64_t fp8_width) {
+int check_norm(const Tensor& x, const OptTensor& w, const OptTensor& r, double eps, int64_t fp8_width) {
   check_rows(x, "x");
-  const int64_t n = x.size(0), d = x.size(1);
+  const SymInt d = x.sym_size(1);
   const int code = code_of(x.scalar_type(), "x");
   TORCH_CHECK_VALUE(d <= MAX_WIDTH && fp8_width <= MAX_WIDTH, "rms_norm takes up to ", MAX_WIDTH,
                     " columns, got ", d);
   TORCH_CHECK_VALUE(eps >= 0 && std::isfinite(eps), "eps must be finite and not negative, got ", eps);
-  TORCH_CHECK(fp8_width == 0 || (fp8_width % 32 == 0 && fp8_width >= d), "tdc.rms_norm: fp8 width");
+  TORCH_CHECK(fp8_width == 0 || (fp8_width % 32 == 0 && d <= fp8_width), "tdc.rms_norm: fp8 width");
   if (has(r)) check_like(*r, x, "residual");
+  check_weights(w, x, {d}, "weight");
+  return code;
+}
+
+std::vector<Tensor> norm_impl(const Tensor& x, const OptTensor& w, const OptTensor& r, double eps,
+                              bool want_rstd, int64_t fp8_width) {
+  const int code = check_norm(x, w, r, eps, fp8_width);
+  const int64_t n = x.size(0), d = x.size(1);
   bool w32;
-  const void* wp = weights_of(w, x, {d}, "weight", w32);
+  const void* wp = weights_of(w, w32);
   const DevGuard guard(x.device());
   std::vector<Tensor> res;
   Tensor q, s, y;
@@ -161,12 +170,13 @@ std::vector<Tensor> rms_norm_bwd(const Tensor& h, const OptTensor& w, const Tens
   if (has(dh)) check_like(*dh, h, "dh");
   const int64_t n = h.size(0), d = h.size(1);
   const int code = code_of(h.scalar_type(), "h");
+  check_weights(w, h, {SymInt(d)}, "weight");
   TORCH_CHECK(d >= 1 && d <= MAX_WIDTH, "tdc.rms_norm_bwd: width");
   TORCH_CHECK(rstd.device() == h.device() && rstd.scalar_type() == at::kFloat &&
                   rstd.is_contiguous() && rstd.numel() == n, "tdc.rms_norm_bwd: rstd fp32 [N]");
   TORCH_CHECK(!want_dw || has(w), "tdc.rms_norm_bwd: dw needs the weights");
   bool w32;
-  const void* wp = weights_of(w, h, {d}, "weight", w32);
+  const void* wp = weights_of(w, w32);
   const DevGuard guard(h.device());
   Tensor dx = fresh({n, d}, h.scalar_type(), h);
   std::vector<Tensor> res = {dx};
@@ -203,34 +213,44 @@ Tensor dequant_fp8(const Tensor& q, const Tensor& s, int64_t d, at::ScalarType d
 }
 
 // ------------------------------------------------------------------ gate
+void check_mask(const OptTensor& mask, const Tensor& scores) {
+  if (!has(mask)) return;
+  TORCH_CHECK_VALUE(mask->scalar_type() == at::kBool, "mask must be a bool tensor");
+  TORCH_CHECK_VALUE(mask->device() == scores.device(), "mask is on ", mask->device(),
+                    ", the scores on ", scores.device());
+  TORCH_CHECK_VALUE(mask->sym_sizes() == scores.sym_sizes(), "mask must be [N, K], got ",
+                    mask->sym_sizes());
+}
+
 struct MaskArg {
   const uint8_t* p = nullptr;
   int64_t rs = 0, cs = 0;
 };
 
-MaskArg mask_of(const OptTensor& mask, const Tensor& like, int64_t n, int64_t K) {
+MaskArg mask_of(const OptTensor& mask) {
   MaskArg m;
   if (!has(mask)) return m;
-  TORCH_CHECK_VALUE(mask->scalar_type() == at::kBool, "mask must be a bool tensor");
-  TORCH_CHECK_VALUE(mask->device() == like.device(), "mask is on ", mask->device(),
-                    ", the scores on ", like.device());
-  TORCH_CHECK_VALUE(mask->dim() == 2 && mask->size(0) == n && mask->size(1) == K,
-                    "mask must be [N, K], got ", mask->sizes());
   m.p = static_cast<const uint8_t*>(mask->data_ptr());
   m.rs = mask->stride(0);
   m.cs = mask->stride(1);
   return m;
 }
 
+int check_gate(const Tensor& scores, const OptTensor& mask, int64_t k) {
+  check_rows(scores, "scores");
+  const SymInt n = scores.sym_size(0), K = scores.sym_size(1);
+  const int code = code_of(scores.scalar_type(), "scores");
+  TORCH_CHECK_VALUE(k >= 1 && k <= 16 && K >= k, "k must be 1 to ", K.min(16), ", got ", k);
+  TORCH_CHECK_VALUE(K <= (1 << 30) && n <= MAX_SLOTS, "too many scores: ", scores.sym_sizes());
+  check_mask(mask, scores);
+  return code;
+}
+
 std::vector<Tensor> gate_impl(const Tensor& scores, const OptTensor& mask, int64_t k, bool normalize,
                               bool want_stat) {
-  check_rows(scores, "scores");
+  const int code = check_gate(scores, mask, k);
   const int64_t n = scores.size(0), K = scores.size(1);
-  const int code = code_of(scores.scalar_type(), "scores");
-  TORCH_CHECK_VALUE(k >= 1 && k <= std::min<int64_t>(16, K), "k must be 1 to ",
-                    std::min<int64_t>(16, K), ", got ", k);
-  TORCH_CHECK_VALUE(K <= (1 << 30) && n <= MAX_SLOTS, "too many scores: ", scores.sizes());
-  const MaskArg m = mask_of(mask, scores, n, K);
+  const MaskArg m = mask_of(mask);
   const DevGuard guard(scores.device());
   Tensor w = fresh({n, k}, at::kFloat, scores);
   Tensor labels = fresh({n, k}, at::kInt, scores);
@@ -277,7 +297,8 @@ Tensor topk_gate_bwd(const OptTensor& scores, const OptTensor& mask, const Tenso
                     scores->size(0) == n && scores->size(1) == K, "tdc.topk_gate_bwd: scores");
     TORCH_CHECK(has(stat) && stat->device() == w.device() && stat->scalar_type() == at::kFloat &&
                     stat->is_contiguous() && stat->numel() == 2 * n, "tdc.topk_gate_bwd: stat");
-    m = mask_of(mask, *scores, n, K);
+    check_mask(mask, *scores);
+    m = mask_of(mask);
   }
   const DevGuard guard(w.device());
   Tensor ds = fresh({n, K}, dtype, w);
@@ -291,15 +312,20 @@ Tensor topk_gate_bwd(const OptTensor& scores, const OptTensor& mask, const Tenso
 }
 
 // ------------------------------------------------------------------ groups
-std::vector<Tensor> group_plan(const Tensor& given, int64_t K) {
+void check_plan(const Tensor& given, int64_t K) {
   TORCH_CHECK_VALUE((given.dim() == 1 || given.dim() == 2) &&
                         (given.scalar_type() == at::kInt || given.scalar_type() == at::kLong),
                     "labels must be int32 or int64 [N] or [N, k], got ", given.scalar_type(), " ",
-                    given.sizes());
-  TORCH_CHECK_VALUE(given.dim() == 1 || given.size(1) >= 1, "labels have no columns");
+                    given.sym_sizes());
+  TORCH_CHECK_VALUE(given.dim() == 1 || given.sym_size(1) >= 1, "labels have no columns");
   TORCH_CHECK_VALUE(K >= 1 && K < (1 << 22), "n_clusters must be 1 to ", (1 << 22) - 1, ", got ", K);
+  TORCH_CHECK_VALUE(given.sym_numel() <= MAX_SLOTS, "at most ", MAX_SLOTS, " labels, got ",
+                    given.sym_numel());
+}
+
+std::vector<Tensor> group_plan(const Tensor& given, int64_t K) {
+  check_plan(given, K);
   const int64_t m = given.numel();
-  TORCH_CHECK_VALUE(m <= MAX_SLOTS, "at most ", MAX_SLOTS, " labels, got ", m);
   const Tensor labels = given.contiguous();
   const DevGuard guard(labels.device());
   Tensor offsets = fresh({K + 1}, at::kInt, labels);
@@ -316,21 +342,30 @@ std::vector<Tensor> group_plan(const Tensor& given, int64_t K) {
 }
 
 // pos int32 [N, k] or [N]: the slots of each row.
-int64_t slots_of(const Tensor& offsets, const Tensor& pos, const Tensor& like) {
-  TORCH_CHECK((pos.dim() == 1 || pos.dim() == 2) && offsets.dim() == 1 && offsets.numel() >= 2,
+SymInt slots_of(const Tensor& offsets, const Tensor& pos, const Tensor& like) {
+  TORCH_CHECK((pos.dim() == 1 || pos.dim() == 2) && offsets.dim() == 1 && offsets.sym_numel() >= 2,
               "tdc: pos [N] or [N, k], offsets [K + 1]");
-  check_index(offsets, like, offsets.numel(), "offsets");
-  check_index(pos, like, pos.numel(), "pos");
-  TORCH_CHECK(pos.numel() <= MAX_SLOTS, "tdc: too many slots");
-  return pos.dim() == 1 ? 1 : pos.size(1);
+  check_index(offsets, like, offsets.sym_numel(), "offsets");
+  check_index(pos, like, pos.sym_numel(), "pos");
+  TORCH_CHECK(pos.sym_numel() <= MAX_SLOTS, "tdc: too many slots");
+  return pos.dim() == 1 ? SymInt(1) : pos.sym_size(1);
+}
+int64_t slots(const Tensor& pos) { return pos.dim() == 1 ? 1 : pos.size(1); }
+
+int check_group(const Tensor& x, const Tensor& offsets, const Tensor& pos) {
+  check_rows(x, "x");
+  slots_of(offsets, pos, x);
+  const int code = code_of(x.scalar_type(), "x");
+  TORCH_CHECK_VALUE(pos.sym_size(0) == x.sym_size(0), "the plan is of ", pos.sym_size(0),
+                    " rows, x has ", x.sym_size(0));
+  TORCH_CHECK_VALUE(x.sym_size(1) <= MAX_COLUMNS, "at most ", MAX_COLUMNS, " columns, got ",
+                    x.sym_size(1));
+  return code;
 }
 
 Tensor group_rows(const Tensor& x, const Tensor& offsets, const Tensor& pos) {
-  check_rows(x, "x");
-  const int64_t n = x.size(0), d = x.size(1), k = slots_of(offsets, pos, x);
-  const int code = code_of(x.scalar_type(), "x");
-  TORCH_CHECK_VALUE(pos.size(0) == n, "the plan is of ", pos.size(0), " rows, x has ", n);
-  TORCH_CHECK_VALUE(d <= MAX_COLUMNS, "at most ", MAX_COLUMNS, " columns, got ", d);
+  const int code = check_group(x, offsets, pos);
+  const int64_t n = x.size(0), d = x.size(1), k = slots(pos);
   const DevGuard guard(x.device());
   Tensor out = fresh({n * k, d}, x.scalar_type(), x);
   check(tdc_group_rows(code, x.data_ptr(), x.stride(0), n, (int)k, (int)d,
@@ -340,15 +375,23 @@ Tensor group_rows(const Tensor& x, const Tensor& offsets, const Tensor& pos) {
   return out;
 }
 
-Tensor combine_rows(const Tensor& y, const Tensor& offsets, const Tensor& pos, const OptTensor& w) {
+int check_combine(const Tensor& y, const Tensor& offsets, const Tensor& pos, const OptTensor& w) {
   check_rows(y, "y");
-  const int64_t n = pos.size(0), d = y.size(1), k = slots_of(offsets, pos, y);
+  const SymInt places = slots_of(offsets, pos, y) * pos.sym_size(0);
   const int code = code_of(y.scalar_type(), "y");
-  TORCH_CHECK_VALUE(y.size(0) == n * k, "the plan is of ", n * k, " places, y has ", y.size(0),
-                    " rows");
-  TORCH_CHECK_VALUE(d <= MAX_COLUMNS, "at most ", MAX_COLUMNS, " columns, got ", d);
+  TORCH_CHECK_VALUE(y.sym_size(0) == places, "the plan is of ", places, " places, y has ",
+                    y.sym_size(0), " rows");
+  TORCH_CHECK_VALUE(y.sym_size(1) <= MAX_COLUMNS, "at most ", MAX_COLUMNS, " columns, got ",
+                    y.sym_size(1));
+  check_weights(w, y, pos.sym_sizes(), "weights");
+  return code;
+}
+
+Tensor combine_rows(const Tensor& y, const Tensor& offsets, const Tensor& pos, const OptTensor& w) {
+  const int code = check_combine(y, offsets, pos, w);
+  const int64_t n = pos.size(0), d = y.size(1), k = slots(pos);
   bool w32;
-  const void* wp = weights_of(w, y, pos.sizes(), "weights", w32);
+  const void* wp = weights_of(w, w32);
   const DevGuard guard(y.device());
   Tensor out = fresh({n, d}, y.scalar_type(), y);
   check(tdc_combine_rows(code, y.data_ptr(), y.stride(0), n, (int)k, (int)d,
@@ -362,12 +405,14 @@ Tensor combine_rows(const Tensor& y, const Tensor& offsets, const Tensor& pos, c
 std::vector<Tensor> combine_rows_bwd(const Tensor& dout, const OptTensor& y, const Tensor& offsets,
                                      const Tensor& pos, const OptTensor& w, bool want_dy) {
   check_rows(dout, "dout");
-  const int64_t n = dout.size(0), d = dout.size(1), k = slots_of(offsets, pos, dout);
+  slots_of(offsets, pos, dout);
+  const int64_t n = dout.size(0), d = dout.size(1), k = slots(pos);
   const int code = code_of(dout.scalar_type(), "dout");
   TORCH_CHECK(pos.size(0) == n && d >= 1 && d <= MAX_SLOTS,
               "tdc.combine_rows_bwd: rows do not fit the plan");
+  check_weights(w, dout, pos.sym_sizes(), "weights");
   bool w32;
-  const void* wp = weights_of(w, dout, pos.sizes(), "weights", w32);
+  const void* wp = weights_of(w, w32);
   const bool want_dw = has(y);
   if (want_dw) {
     check_rows(*y, "y");
@@ -395,6 +440,88 @@ std::vector<Tensor> combine_rows_bwd(const Tensor& dout, const OptTensor& y, con
   return res;
 }
 
+// ------------------------------------------------------------------ shapes
+// The results of each operator as tensors without data: what tracing and compilation run in
+// the kernels' place.
+Tensor shaped(c10::SymIntArrayRef sizes, at::ScalarType t, const Tensor& like) {
+  return at::empty_symint(sizes, at::TensorOptions().dtype(t).device(like.device()));
+}
+
+std::vector<Tensor> norm_shapes(const Tensor& x, const OptTensor& w, const OptTensor& r, double eps,
+                                bool want_rstd, int64_t fp8_width) {
+  check_norm(x, w, r, eps, fp8_width);
+  const SymInt n = x.sym_size(0), d = x.sym_size(1);
+  std::vector<Tensor> res;
+  if (fp8_width) {
+    res = {shaped({n, fp8_width}, at::kFloat8_e4m3fn, x), shaped({n, fp8_width / 32}, at::kByte, x)};
+  } else {
+    res = {shaped({n, d}, x.scalar_type(), x)};
+  }
+  if (has(r)) res.push_back(shaped({n, d}, x.scalar_type(), x));
+  if (want_rstd) res.push_back(shaped({n}, at::kFloat, x));
+  return res;
+}
+std::vector<Tensor> rms_norm_shapes(const Tensor& x, const OptTensor& w, const OptTensor& r,
+                                    double eps) {
+  return norm_shapes(x, w, r, eps, false, 0);
+}
+std::vector<Tensor> rms_norm_train_shapes(const Tensor& x, const OptTensor& w, const OptTensor& r,
+                                          double eps) {
+  return norm_shapes(x, w, r, eps, true, 0);
+}
+std::vector<Tensor> rms_norm_fp8_shapes(const Tensor& x, const OptTensor& w, const OptTensor& r,
+                                        double eps, int64_t width) {
+  return norm_shapes(x, w, r, eps, false, width);
+}
+std::vector<Tensor> rms_norm_bwd_shapes(const Tensor& h, const OptTensor& w, const Tensor&,
+                                        const Tensor&, const OptTensor&, bool want_dw) {
+  std::vector<Tensor> res = {shaped(h.sym_sizes(), h.scalar_type(), h)};
+  if (want_dw) res.push_back(shaped(w->sym_sizes(), w->scalar_type(), *w));
+  return res;
+}
+Tensor dequant_fp8_shapes(const Tensor& q, const Tensor&, SymInt d, at::ScalarType dtype) {
+  return shaped({q.sym_size(0), std::move(d)}, dtype, q);
+}
+
+std::tuple<Tensor, Tensor> topk_gate_shapes(const Tensor& scores, const OptTensor& mask, int64_t k,
+                                            bool) {
+  check_gate(scores, mask, k);
+  const SymInt n = scores.sym_size(0);
+  return {shaped({n, k}, at::kFloat, scores), shaped({n, k}, at::kInt, scores)};
+}
+std::vector<Tensor> topk_gate_train_shapes(const Tensor& scores, const OptTensor& mask, int64_t k,
+                                           bool normalize) {
+  const auto [w, labels] = topk_gate_shapes(scores, mask, k, normalize);
+  if (normalize) return {w, labels};
+  return {w, labels, shaped({scores.sym_size(0), 2}, at::kFloat, scores)};
+}
+Tensor topk_gate_bwd_shapes(const OptTensor&, const OptTensor&, const Tensor& w, const Tensor&,
+                            const OptTensor&, const Tensor&, SymInt K, at::ScalarType dtype) {
+  return shaped({w.sym_size(0), std::move(K)}, dtype, w);
+}
+
+std::vector<Tensor> group_plan_shapes(const Tensor& labels, int64_t K) {
+  check_plan(labels, K);
+  return {shaped({K + 1}, at::kInt, labels), shaped({labels.sym_numel()}, at::kInt, labels),
+          shaped(labels.sym_sizes(), at::kInt, labels)};
+}
+Tensor group_rows_shapes(const Tensor& x, const Tensor& offsets, const Tensor& pos) {
+  check_group(x, offsets, pos);
+  return shaped({pos.sym_numel(), x.sym_size(1)}, x.scalar_type(), x);
+}
+Tensor combine_rows_shapes(const Tensor& y, const Tensor& offsets, const Tensor& pos,
+                           const OptTensor& w) {
+  check_combine(y, offsets, pos, w);
+  return shaped({pos.sym_size(0), y.sym_size(1)}, y.scalar_type(), y);
+}
+std::vector<Tensor> combine_rows_bwd_shapes(const Tensor& dout, const OptTensor& y, const Tensor&,
+                                            const Tensor& pos, const OptTensor& w, bool want_dy) {
+  std::vector<Tensor> res;
+  if (want_dy) res.push_back(shaped({pos.sym_numel(), dout.sym_size(1)}, dout.scalar_type(), dout));
+  if (has(y)) res.push_back(shaped(w->sym_sizes(), w->scalar_type(), *w));
+  return res;
+}
+
 // ------------------------------------------------------------------ autograd
 using torch::autograd::AutogradContext;
 using torch::autograd::Function;
@@ -402,11 +529,11 @@ using torch::autograd::variable_list;
 
 // The operator tdc::NAME below autograd, with the signature of its kernel.  Not the kernel
 // itself: what stands between the two (dispatch modes, tracing) sees the call as it sees
-// PyTorch's own (0.5 us of a call).
+// PyTorch's own (0.1 us of a call).
 #define TDC_BELOW_AUTOGRAD(NAME, ...)                                                     \
   [&] {                                                                                   \
     static const auto op =                                                                \
-        c10::Dispatcher::singleton().findSchemaOrThrow("tdc::" #NAME, "").typed<decltype(NAME)>(); \
+        c10::Dispatcher::singleton().findSchemaOrThrow("tdc::" #NAME, "").typed<decltype(NAME##_shapes)>(); \
     const at::AutoDispatchBelowADInplaceOrView below;                                     \
     return op.call(__VA_ARGS__);                                                          \
   }()
@@ -416,7 +543,7 @@ bool wants_grad(const OptTensor& t) { return has(t) && t->requires_grad(); }
 
 // An incoming gradient in a layout that the kernels take (broadcast ones are laid out).
 Tensor laid_out(const Tensor& g) {
-  if (!g.defined() || g.size(1) <= 1 || g.stride(1) == 1) return g;
+  if (!g.defined() || g.sym_size(1) <= 1 || g.sym_stride(1) == 1) return g;
   return g.contiguous();
 }
 
@@ -509,7 +636,7 @@ struct TopkGate : public Function<TopkGate> {
       ctx->save_for_backward({out[0], out[1]});
     else
       ctx->save_for_backward({out[0], out[1], scores, out[2], has(mask) ? *mask : Tensor()});
-    ctx->saved_data["clusters"] = scores.size(1);
+    ctx->saved_data["clusters"] = scores.sym_size(1);
     ctx->saved_data["dtype"] = (int64_t)scores.scalar_type();
     return {out[0], out[1]};
   }
@@ -523,7 +650,7 @@ struct TopkGate : public Function<TopkGate> {
     res[0] = TDC_BELOW_AUTOGRAD(topk_gate_bwd, normalize ? none : opt(saved[2]),
                                 normalize ? none : opt(saved[4]), saved[0], saved[1],
                                 normalize ? none : opt(saved[3]), grads[0].contiguous(),
-                                ctx->saved_data["clusters"].toInt(),
+                                ctx->saved_data["clusters"].toSymInt(),
                                 (at::ScalarType)ctx->saved_data["dtype"].toInt());
     return once(res, grads, saved);
   }
@@ -622,7 +749,7 @@ Tensor combine_rows_ad(const Tensor& y, const Tensor& offsets, const Tensor& pos
 TORCH_LIBRARY_FRAGMENT(tdc, m) {
   m.def("rms_norm(Tensor x, Tensor? w, Tensor? r, float eps) -> Tensor[]");
   m.def("rms_norm_fp8(Tensor x, Tensor? w, Tensor? r, float eps, int width) -> Tensor[]");
-  m.def("dequant_fp8(Tensor q, Tensor s, int d, ScalarType dtype) -> Tensor");
+  m.def("dequant_fp8(Tensor q, Tensor s, SymInt d, ScalarType dtype) -> Tensor");
   m.def("topk_gate(Tensor scores, Tensor? mask, int k, bool normalize) -> (Tensor, Tensor)");
   m.def("group_plan(Tensor labels, int K) -> Tensor[]");
   m.def("group_rows(Tensor x, Tensor offsets, Tensor pos) -> Tensor");
@@ -632,7 +759,7 @@ TORCH_LIBRARY_FRAGMENT(tdc, m) {
   m.def("rms_norm_bwd(Tensor h, Tensor? w, Tensor rstd, Tensor dy, Tensor? dh, bool want_dw) -> Tensor[]");
   m.def("topk_gate_train(Tensor scores, Tensor? mask, int k, bool normalize) -> Tensor[]");
   m.def("topk_gate_bwd(Tensor? scores, Tensor? mask, Tensor w, Tensor labels, Tensor? stat, "
-        "Tensor dw, int K, ScalarType dtype) -> Tensor");
+        "Tensor dw, SymInt K, ScalarType dtype) -> Tensor");
   m.def("combine_rows_bwd(Tensor dout, Tensor? y, Tensor offsets, Tensor pos, Tensor? w, "
         "bool want_dy) -> Tensor[]");
 }
@@ -650,6 +777,21 @@ TORCH_LIBRARY_IMPL(tdc, CUDA, m) {
   m.impl("topk_gate_train", &topk_gate_train);
   m.impl("topk_gate_bwd", &topk_gate_bwd);
   m.impl("combine_rows_bwd", &combine_rows_bwd);
+}
+
+TORCH_LIBRARY_IMPL(tdc, Meta, m) {
+  m.impl("rms_norm", &rms_norm_shapes);
+  m.impl("rms_norm_fp8", &rms_norm_fp8_shapes);
+  m.impl("dequant_fp8", &dequant_fp8_shapes);
+  m.impl("topk_gate", &topk_gate_shapes);
+  m.impl("group_plan", &group_plan_shapes);
+  m.impl("group_rows", &group_rows_shapes);
+  m.impl("combine_rows", &combine_rows_shapes);
+  m.impl("rms_norm_train", &rms_norm_train_shapes);
+  m.impl("rms_norm_bwd", &rms_norm_bwd_shapes);
+  m.impl("topk_gate_train", &topk_gate_train_shapes);
+  m.impl("topk_gate_bwd", &topk_gate_bwd_shapes);
+  m.impl("combine_rows_bwd", &combine_rows_bwd_shapes);
 }
 
 TORCH_LIBRARY_IMPL(tdc, AutogradCUDA, m) {

@@ -16,7 +16,8 @@ are differentiable (once, and backward: a GPU tensor with a forward-mode tangent
 NotImplementedError).  Nothing synchronises with the host and every buffer is a new tensor,
 so the calls can be captured into a HIP graph, the gradients too: capture forward and
 backward together, with no other live autograd graph of the same leaves (a captured gradient
-that would go into one raises RuntimeError).
+that would go into one raises RuntimeError).  The operators can be traced and compiled:
+they have shape functions and dispatch as PyTorch's own do.
 """
 from __future__ import annotations
 

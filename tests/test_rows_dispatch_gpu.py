@@ -1,5 +1,5 @@
 """Row operators under PyTorch's own machinery on the GPU: forward-mode gradients, dispatch
-modes, tracing."""
+modes, tracing, compilation."""
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd
@@ -112,7 +112,40 @@ def test_traced_on_one_input_and_run_on_another(gpu, name):
     call, _ = CALLS[name]
     args, other = inputs(gpu, name), inputs(gpu, name, seed=10)
     for f in (lambda *a: tuple_of(call(gpu, *a)), lambda *a: with_grads(gpu, call, a)):
-        graph = make_fx(f, tracing_mode="real")(*args)
-        for given in (args, other):
-            for a, b in zip(graph(*given), f(*given)):
-                assert torch.equal(a, b)
+        for mode in ("real", "fake", "symbolic"):
+            graph = make_fx(f, tracing_mode=mode)(*args)
+            for given in (args, other):
+                for a, b in zip(graph(*given), f(*given)):
+                    assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("name", CALLS)
+@pytest.mark.parametrize("dynamic", [False, True])
+def test_compiled(gpu, name, dynamic):
+    """Forward and backward graphs of the compiler, run by the operators themselves."""
+    call, _ = CALLS[name]
+    compiled = torch.compile(lambda *a: tuple_of(call(gpu, *a)), backend="aot_eager", dynamic=dynamic)
+    for seed in (0, 10):
+        args = inputs(gpu, name, seed)
+        with torch.no_grad():
+            assert all(torch.equal(a, b) for a, b in zip(compiled(*args), tuple_of(call(gpu, *args))))
+        got = with_grads(gpu, lambda gpu, *a: compiled(*a), args)
+        assert all(torch.equal(a, b) for a, b in zip(got, with_grads(gpu, call, args)))
+
+
+def test_registered_as_pytorch_asks(gpu):
+    ops = torch.ops.tdc
+    x, w, s = normal(gpu, 1, 6, 40), normal(gpu, 2, 40), normal(gpu, 3, 6, 9)
+    y, v, groups = normal(gpu, 4, 12, 40), normal(gpu, 5, 6, 2).abs(), plan(gpu)
+    lab, rows = groups.pos % 3, tdc.rms_norm_fp8(x)
+    for t in (x, w, s, y, v):
+        t.requires_grad_()
+    # the other checks multiply fp8 tensors, which PyTorch does not
+    torch.library.opcheck(ops.rms_norm_fp8.default, (x.detach(), None, None, 1e-6, 256), test_utils="test_faketensor")
+    torch.library.opcheck(ops.dequant_fp8.default, (rows.q, rows.scales, 40, torch.float32), test_utils="test_faketensor")
+    for op, args in ((ops.rms_norm, (x, w, None, 1e-6)), (ops.rms_norm, (x, w, y[:6].detach(), 1e-6)),
+                     (ops.topk_gate, (s, None, 3, True)), (ops.topk_gate, (s, s.detach() < 1, 3, False)),
+                     (ops.group_plan, (lab, 3)), (ops.group_rows, (x, groups.offsets, groups.pos)),
+                     (ops.combine_rows, (y, groups.offsets, groups.pos, v))):
+        torch.library.opcheck(op.default, args, test_utils=(
+            "test_schema", "test_autograd_registration", "test_faketensor", "test_aot_dispatch_dynamic"))
