@@ -247,7 +247,7 @@ int check_gate(const Tensor& scores, const OptTensor& mask, int64_t k) {
 }
 
 std::vector<Tensor> gate_impl(const Tensor& scores, const OptTensor& mask, int64_t k, bool normalize,
-                              bool want_stat) {
+                              bool train) {
   const int code = check_gate(scores, mask, k);
   const int64_t n = scores.size(0), K = scores.size(1);
   const MaskArg m = mask_of(mask);
@@ -255,13 +255,18 @@ std::vector<Tensor> gate_impl(const Tensor& scores, const OptTensor& mask, int64
   Tensor w = fresh({n, k}, at::kFloat, scores);
   Tensor labels = fresh({n, k}, at::kInt, scores);
   std::vector<Tensor> res = {w, labels};
-  Tensor stat;
-  if (want_stat) {
-    stat = fresh({n, 2}, at::kFloat, scores);
-    res.push_back(stat);
+  Tensor chosen, stat;
+  if (train) {
+    chosen = fresh({n, k, 2}, at::kInt, scores);
+    res.push_back(chosen);
+    if (!normalize) {
+      stat = fresh({n, 2}, at::kFloat, scores);
+      res.push_back(stat);
+    }
   }
   check(tdc_topk_gate(code, scores.data_ptr(), scores.stride(0), m.p, m.rs, m.cs, n, (int)K, (int)k,
                       normalize, w.data_ptr<float>(), labels.data_ptr<int32_t>(),
+                      chosen.defined() ? chosen.data_ptr() : nullptr,
                       stat.defined() ? stat.data_ptr<float>() : nullptr, cur_stream()),
         "topk_gate");
   return res;
@@ -272,39 +277,38 @@ std::tuple<Tensor, Tensor> topk_gate(const Tensor& scores, const OptTensor& mask
   const std::vector<Tensor> out = gate_impl(scores, mask, k, normalize, false);
   return {out[0], out[1]};
 }
-// with what the gradient over all clusters needs: w, labels[, stat]
+// with what the gradient needs: w, labels, both again as pairs int32 [N, k, 2][, stat]
 std::vector<Tensor> topk_gate_train(const Tensor& scores, const OptTensor& mask, int64_t k,
                                     bool normalize) {
-  return gate_impl(scores, mask, k, normalize, !normalize);
+  return gate_impl(scores, mask, k, normalize, true);
 }
 
 // scores, mask, stat: given without `normalize` only.
-Tensor topk_gate_bwd(const OptTensor& scores, const OptTensor& mask, const Tensor& w,
-                     const Tensor& labels, const OptTensor& stat, const Tensor& dw, int64_t K,
-                     at::ScalarType dtype) {
-  TORCH_CHECK(w.is_cuda() && w.dim() == 2 && w.scalar_type() == at::kFloat && w.is_contiguous(),
-              "tdc.topk_gate_bwd: w fp32 [N, k]");
-  const int64_t n = w.size(0), k = w.size(1);
-  check_index(labels, w, n * k, "labels");
-  TORCH_CHECK(dw.device() == w.device() && dw.scalar_type() == at::kFloat && dw.is_contiguous() &&
+Tensor topk_gate_bwd(const OptTensor& scores, const OptTensor& mask, const Tensor& chosen,
+                     const OptTensor& stat, const Tensor& dw, int64_t K, at::ScalarType dtype) {
+  TORCH_CHECK(chosen.is_cuda() && chosen.dim() == 3 && chosen.size(2) == 2 &&
+                  chosen.scalar_type() == at::kInt && chosen.is_contiguous(),
+              "tdc.topk_gate_bwd: chosen int32 [N, k, 2]");
+  const int64_t n = chosen.size(0), k = chosen.size(1);
+  TORCH_CHECK(dw.device() == chosen.device() && dw.scalar_type() == at::kFloat && dw.is_contiguous() &&
                   dw.numel() == n * k, "tdc.topk_gate_bwd: dw fp32 [N, k]");
   const int code = code_of(dtype, "scores");
   const bool normalize = !has(scores);
   MaskArg m;
   if (!normalize) {
     check_rows(*scores, "scores");
-    TORCH_CHECK(scores->device() == w.device() && scores->scalar_type() == dtype &&
+    TORCH_CHECK(scores->device() == chosen.device() && scores->scalar_type() == dtype &&
                     scores->size(0) == n && scores->size(1) == K, "tdc.topk_gate_bwd: scores");
-    TORCH_CHECK(has(stat) && stat->device() == w.device() && stat->scalar_type() == at::kFloat &&
-                    stat->is_contiguous() && stat->numel() == 2 * n, "tdc.topk_gate_bwd: stat");
+    TORCH_CHECK(has(stat) && stat->device() == chosen.device() &&
+                    stat->scalar_type() == at::kFloat && stat->is_contiguous() && stat->numel() == 2 * n, "tdc.topk_gate_bwd: stat");
     check_mask(mask, *scores);
     m = mask_of(mask);
   }
-  const DevGuard guard(w.device());
-  Tensor ds = fresh({n, K}, dtype, w);
+  const DevGuard guard(chosen.device());
+  Tensor ds = fresh({n, K}, dtype, chosen);
   check(tdc_topk_gate_bwd(code, normalize ? nullptr : scores->data_ptr(),
-                          normalize ? 0 : scores->stride(0), m.p, m.rs, m.cs, w.data_ptr<float>(),
-                          labels.data_ptr<int32_t>(), normalize ? nullptr : stat->data_ptr<float>(),
+                          normalize ? 0 : scores->stride(0), m.p, m.rs, m.cs, chosen.data_ptr(),
+                          normalize ? nullptr : stat->data_ptr<float>(),
                           dw.data_ptr<float>(), n, (int)K, (int)k, normalize, ds.data_ptr(),
                           cur_stream()),
         "topk_gate_bwd");
@@ -492,12 +496,14 @@ std::tuple<Tensor, Tensor> topk_gate_shapes(const Tensor& scores, const OptTenso
 std::vector<Tensor> topk_gate_train_shapes(const Tensor& scores, const OptTensor& mask, int64_t k,
                                            bool normalize) {
   const auto [w, labels] = topk_gate_shapes(scores, mask, k, normalize);
-  if (normalize) return {w, labels};
-  return {w, labels, shaped({scores.sym_size(0), 2}, at::kFloat, scores)};
+  const SymInt n = scores.sym_size(0);
+  const Tensor chosen = shaped({n, k, 2}, at::kInt, scores);
+  if (normalize) return {w, labels, chosen};
+  return {w, labels, chosen, shaped({n, 2}, at::kFloat, scores)};
 }
-Tensor topk_gate_bwd_shapes(const OptTensor&, const OptTensor&, const Tensor& w, const Tensor&,
+Tensor topk_gate_bwd_shapes(const OptTensor&, const OptTensor&, const Tensor& chosen,
                             const OptTensor&, const Tensor&, SymInt K, at::ScalarType dtype) {
-  return shaped({w.sym_size(0), std::move(K)}, dtype, w);
+  return shaped({chosen.sym_size(0), std::move(K)}, dtype, chosen);
 }
 
 std::vector<Tensor> group_plan_shapes(const Tensor& labels, int64_t K) {
@@ -589,6 +595,20 @@ void check_capture() {
   }
 }
 
+// Stand-ins for the inputs of the node that runs, for `once`: the gate's gradient is made from
+// copies that no longer lead back to its scores.
+variable_list inputs_of_node() {
+  variable_list res;
+  const auto node = torch::autograd::get_current_node();
+  if (!node || !at::GradMode::is_enabled()) return res;
+  for (const auto& edge : node->next_edges()) {
+    if (!edge.is_valid()) continue;
+    res.push_back(at::empty({0}, at::kFloat));
+    torch::autograd::impl::set_gradient_edge(res.back(), edge);
+  }
+  return res;
+}
+
 OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; }
 
 struct RmsNorm : public Function<RmsNorm> {
@@ -630,12 +650,12 @@ struct TopkGate : public Function<TopkGate> {
     std::vector<Tensor> out = TDC_BELOW_AUTOGRAD(topk_gate_train, scores, mask, k, normalize);
     ctx->set_materialize_grads(false);
     ctx->mark_non_differentiable({out[1]});
-    // the weights over the chosen say all about their gradient; those over every cluster
-    // need the scores again
+    // not the outputs, which the caller may edit; the weights over the chosen say all about
+    // their gradient, those over every cluster need the scores again
     if (normalize)
-      ctx->save_for_backward({out[0], out[1]});
+      ctx->save_for_backward({out[2]});
     else
-      ctx->save_for_backward({out[0], out[1], scores, out[2], has(mask) ? *mask : Tensor()});
+      ctx->save_for_backward({out[2], scores, out[3], has(mask) ? *mask : Tensor()});
     ctx->saved_data["clusters"] = scores.sym_size(1);
     ctx->saved_data["dtype"] = (int64_t)scores.scalar_type();
     return {out[0], out[1]};
@@ -645,14 +665,14 @@ struct TopkGate : public Function<TopkGate> {
     variable_list res(4);
     if (!grads[0].defined()) return res;
     const auto saved = ctx->get_saved_variables();
-    const bool normalize = saved.size() == 2;
+    const bool normalize = saved.size() == 1;
     const OptTensor none;
-    res[0] = TDC_BELOW_AUTOGRAD(topk_gate_bwd, normalize ? none : opt(saved[2]),
-                                normalize ? none : opt(saved[4]), saved[0], saved[1],
-                                normalize ? none : opt(saved[3]), grads[0].contiguous(),
+    res[0] = TDC_BELOW_AUTOGRAD(topk_gate_bwd, normalize ? none : opt(saved[1]),
+                                normalize ? none : opt(saved[3]), saved[0],
+                                normalize ? none : opt(saved[2]), grads[0].contiguous(),
                                 ctx->saved_data["clusters"].toSymInt(),
                                 (at::ScalarType)ctx->saved_data["dtype"].toInt());
-    return once(res, grads, saved);
+    return once(res, grads, inputs_of_node());
   }
 };
 
@@ -758,8 +778,8 @@ TORCH_LIBRARY_FRAGMENT(tdc, m) {
   m.def("rms_norm_train(Tensor x, Tensor? w, Tensor? r, float eps) -> Tensor[]");
   m.def("rms_norm_bwd(Tensor h, Tensor? w, Tensor rstd, Tensor dy, Tensor? dh, bool want_dw) -> Tensor[]");
   m.def("topk_gate_train(Tensor scores, Tensor? mask, int k, bool normalize) -> Tensor[]");
-  m.def("topk_gate_bwd(Tensor? scores, Tensor? mask, Tensor w, Tensor labels, Tensor? stat, "
-        "Tensor dw, SymInt K, ScalarType dtype) -> Tensor");
+  m.def("topk_gate_bwd(Tensor? scores, Tensor? mask, Tensor chosen, Tensor? stat, Tensor dw, "
+        "SymInt K, ScalarType dtype) -> Tensor");
   m.def("combine_rows_bwd(Tensor dout, Tensor? y, Tensor offsets, Tensor pos, Tensor? w, "
         "bool want_dy) -> Tensor[]");
 }

@@ -252,17 +252,18 @@ int tdc_rms_norm_bwd(int dtype, const void* h, int64_t ldh, const float* rstd, c
 // out [n, d] = q 2^(s - 127)
 int tdc_dequant_fp8(int dtype, const void* q, const void* s, int64_t n, int d, int dp, void* out,
                     hipStream_t stream);
-// Top-k gate (rows_gate.hip), k <= 16: w fp32 [n, k], labels int32 [n, k] (-1: none), stat
-// (nullable) fp32 [n, 2] = largest score, 1 / sum of exponentials; mask (nullable) bytes,
-// nonzero = allowed, with row and column strides.
+// Top-k gate (rows_gate.hip), k <= 16: w fp32 [n, k], labels int32 [n, k] (-1: none), chosen
+// (nullable) [n, k] pairs of both for the gradient, stat (nullable) fp32 [n, 2] = largest
+// score, 1 / sum of exponentials; mask (nullable) bytes, nonzero = allowed, with row and
+// column strides.
 int tdc_topk_gate(int dtype, const void* scores, int64_t ld, const uint8_t* mask, int64_t mask_rs,
                   int64_t mask_cs, int64_t n, int K, int k, int normalize, float* w, int* labels,
-                  float* stat, hipStream_t stream);
+                  void* chosen, float* stat, hipStream_t stream);
 // ds [n, K] in the scores' type; scores, mask and stat are read without normalize only.
 int tdc_topk_gate_bwd(int dtype, const void* scores, int64_t ld, const uint8_t* mask,
-                      int64_t mask_rs, int64_t mask_cs, const float* w, const int* labels,
-                      const float* stat, const float* dw, int64_t n, int K, int k, int normalize,
-                      void* ds, hipStream_t stream);
+                      int64_t mask_rs, int64_t mask_cs, const void* chosen, const float* stat,
+                      const float* dw, int64_t n, int K, int k, int normalize, void* ds,
+                      hipStream_t stream);
 // Plan of rows by cluster (rows_group.hip): stable sort of m slots by label (int32, or int64
 // with wide_labels), K < 2^22; order / pos int32 [m], offsets int32 [K + 1]; work: int32
 // [tdc_group_plan_work(m, K)].

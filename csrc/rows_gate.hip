@@ -138,11 +138,21 @@ template <int R> constexpr int column(int i, int v, int L, int lane) {
   return ((i / v) * L + lane) * v + i % v;
 }
 
+// One choice of a row.  `chosen` (label, weight): what the gradient goes by, apart from the
+// caller's tensors, which a router edits (labels over a capacity become -1).
+__device__ __forceinline__ void store_choice(int at, float weight, int64_t i, float* __restrict__ w,
+                                             int* __restrict__ labels, int2* __restrict__ chosen) {
+  w[i] = weight;
+  labels[i] = at;
+  if (chosen) chosen[i] = make_int2(at, __float_as_int(weight));
+}
+
 template <typename T, int L, int R, int TAIL, bool MASKED>
 __global__ __launch_bounds__(GATE_BLOCK) void gate_kernel(const T* __restrict__ scores, int64_t ld,
                                                           Mask mask, int64_t n, int K, int k,
                                                           bool normalize, float* __restrict__ w,
                                                           int* __restrict__ labels,
+                                                          int2* __restrict__ chosen,
                                                           float* __restrict__ stat) {
   constexpr int V = Vec<T>::N;
   constexpr unsigned INDEX = low_bits(L * R);  // the bits of a column
@@ -258,10 +268,7 @@ __global__ __launch_bounds__(GATE_BLOCK) void gate_kernel(const T* __restrict__ 
     for (int i = 0; i < R; ++i) sum += num[i] > NONE ? expf(v[i] - first) : 0.f;
   }
   sum = __uint_as_float(group_all<L>(__float_as_uint(sum), Sum(), s_all, turn));
-  if (lane < k) {
-    w[row * k + lane] = at >= 0 ? e / sum : 0.f;
-    labels[row * k + lane] = at;
-  }
+  if (lane < k) store_choice(at, at >= 0 ? e / sum : 0.f, row * k + lane, w, labels, chosen);
   if (stat && lane == 0) {
     stat[2 * row] = first;
     stat[2 * row + 1] = at >= 0 ? 1.f / sum : 0.f;
@@ -275,7 +282,8 @@ __global__ __launch_bounds__(GATE_BLOCK) void gate_kernel(const T* __restrict__ 
 template <typename T, int TAIL, bool MASKED>
 __global__ __launch_bounds__(GATE_BLOCK) void gate_wide_kernel(
     const T* __restrict__ scores, int64_t ld, Mask mask, int64_t n, int K, int k, bool normalize,
-    float* __restrict__ w, int* __restrict__ labels, float* __restrict__ stat) {
+    float* __restrict__ w, int* __restrict__ labels, int2* __restrict__ chosen,
+    float* __restrict__ stat) {
   constexpr int V = Vec<T>::N, L = GATE_BLOCK, R = 32;
   __shared__ unsigned s_all[2][4];
   int turn = 0;
@@ -353,10 +361,8 @@ __global__ __launch_bounds__(GATE_BLOCK) void gate_wide_kernel(
     total = lanes_sum<64>(e);
   else
     total = __uint_as_float(group_all<L>(__float_as_uint(total), Sum(), s_all, turn));
-  if ((int)threadIdx.x < k) {
-    w[row * k + threadIdx.x] = list ? e / total : 0.f;
-    labels[row * k + threadIdx.x] = at;
-  }
+  if ((int)threadIdx.x < k)
+    store_choice(at, list ? e / total : 0.f, row * k + threadIdx.x, w, labels, chosen);
   if (stat && threadIdx.x == 0) {
     stat[2 * row] = first;
     stat[2 * row + 1] = top ? 1.f / total : 0.f;
@@ -369,8 +375,8 @@ __global__ __launch_bounds__(GATE_BLOCK) void gate_wide_kernel(
 // 17.6 us, bound by its 67 MB of stores and the latency of the few loads before them.
 template <typename T, int L, int TAIL>
 __global__ __launch_bounds__(GATE_BLOCK) void gate_bwd_kernel(
-    const T* __restrict__ scores, int64_t ld, Mask mask, const float* __restrict__ w,
-    const int* __restrict__ labels, const float* __restrict__ stat, const float* __restrict__ dw,
+    const T* __restrict__ scores, int64_t ld, Mask mask, const int2* __restrict__ chosen,
+    const float* __restrict__ stat, const float* __restrict__ dw,
     int64_t n, int K, int k, bool normalize, T* __restrict__ ds) {
   constexpr int V = Vec<T>::N, U = 16 / V;
   constexpr int PASS = L * V * U;  // columns
@@ -379,9 +385,10 @@ __global__ __launch_bounds__(GATE_BLOCK) void gate_bwd_kernel(
   float* mine = more[threadIdx.x / L];
   const int64_t row = block_index() * (GATE_BLOCK / L) + threadIdx.x / L;
   if (row >= n) return;
-  const float wj = lane < k ? w[row * k + lane] : 0.f;
+  const int2 choice = lane < k ? chosen[row * k + lane] : make_int2(-1, 0);
   const float dj = lane < k ? dw[row * k + lane] : 0.f;
-  const int at = lane < k ? labels[row * k + lane] : -1;
+  const int at = choice.x;
+  const float wj = __int_as_float(choice.y);
   const float top = normalize ? 0.f : stat[2 * row];
   const float inv = normalize ? 0.f : stat[2 * row + 1];
   const float mean = lanes_sum<L>(at >= 0 ? wj * dj : 0.f);
@@ -431,7 +438,7 @@ using namespace tdc::rows;
 
 int tdc_topk_gate(int dtype, const void* scores, int64_t ld, const uint8_t* mask, int64_t mask_rs,
                   int64_t mask_cs, int64_t n, int K, int k, int normalize, float* w, int* labels,
-                  float* stat, hipStream_t stream) {
+                  void* chosen, float* stat, hipStream_t stream) {
   if (n == 0) return 0;
   if (k < 1 || k > GATE_MAX_K || K < 1 || n > 0x7fffffff) return (int)hipErrorInvalidValue;
   const Mask m{mask, mask_rs, mask_cs};
@@ -440,7 +447,8 @@ int tdc_topk_gate(int dtype, const void* scores, int64_t ld, const uint8_t* mask
     auto go = [&](auto kernel, int lanes) {
       const int rows = GATE_BLOCK / lanes;
       hipLaunchKernelGGL(kernel, grid_of((n + rows - 1) / rows), dim3(GATE_BLOCK), 0,
-                         stream, (const T*)scores, ld, m, n, K, k, normalize != 0, w, labels, stat);
+                         stream, (const T*)scores, ld, m, n, K, k, normalize != 0, w, labels,
+                         (int2*)chosen, stat);
     };
     return with_tail(K, Vec<T>::N, [&](auto tail) {
       constexpr int TAIL = decltype(tail)::value;
@@ -482,9 +490,9 @@ int tdc_topk_gate(int dtype, const void* scores, int64_t ld, const uint8_t* mask
 }
 
 int tdc_topk_gate_bwd(int dtype, const void* scores, int64_t ld, const uint8_t* mask,
-                      int64_t mask_rs, int64_t mask_cs, const float* w, const int* labels,
-                      const float* stat, const float* dw, int64_t n, int K, int k, int normalize,
-                      void* ds, hipStream_t stream) {
+                      int64_t mask_rs, int64_t mask_cs, const void* chosen, const float* stat,
+                      const float* dw, int64_t n, int K, int k, int normalize, void* ds,
+                      hipStream_t stream) {
   if (n == 0) return 0;
   if (k < 1 || k > GATE_MAX_K || K < 1 || n > 0x7fffffff) return (int)hipErrorInvalidValue;
   const Mask m{mask, mask_rs, mask_cs};
@@ -493,8 +501,8 @@ int tdc_topk_gate_bwd(int dtype, const void* scores, int64_t ld, const uint8_t* 
     auto go = [&](auto kernel, int lanes) {
       const int rows = GATE_BLOCK / lanes;
       hipLaunchKernelGGL(kernel, grid_of((n + rows - 1) / rows), dim3(GATE_BLOCK), 0,
-                         stream, (const T*)scores, ld, m, w, labels, stat, dw, n, K, k,
-                         normalize != 0, (T*)ds);
+                         stream, (const T*)scores, ld, m, (const int2*)chosen, stat, dw, n, K,
+                         k, normalize != 0, (T*)ds);
     };
     return with_tail(K, Vec<T>::N, [&](auto tail) {
       constexpr int TAIL = decltype(tail)::value;

@@ -168,7 +168,8 @@ def topk_gate(scores: torch.Tensor, k: int, mask: Optional[torch.Tensor] = None,
     (``normalize``) or over all allowed clusters.  ``mask`` (bool [N, K], or broadcast to
     it): True where a cluster is allowed; one that is not, and one whose score is -inf, is
     never chosen, its score is not looked at and its gradient is zero.  Where fewer than k
-    are left the last labels are -1 with weight 0, which :func:`group_plan` leaves out.  A
+    are left the last labels are -1 with weight 0, which :func:`group_plan` leaves out.  Both
+    may be edited in place (labels over a capacity set to -1): the gradient keeps its own.  A
     NaN or +inf among the allowed scores makes the row's weights NaN."""
     gpu = _on_gpu(scores, mask)
     k, normalize = int(k), bool(normalize)

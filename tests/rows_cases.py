@@ -135,6 +135,25 @@ def check_dropped_weights(device, bad):
     assert torch.equal(dy, want)
 
 
+def check_gate_edited(device, normalize):
+    """What a router does with its choice: drop labels over a capacity, put the weights right,
+    in place."""
+    g = torch.Generator().manual_seed(1)
+    s, dw = torch.randn(50, 12, generator=g).to(device), torch.randn(50, 3, generator=g).to(device)
+    over = (torch.rand(50, 3, generator=g) < 0.3).to(device)
+    res = []
+    for edit in (True, False):
+        leaf = s.clone().requires_grad_()
+        w, lab = tdc.topk_gate(leaf, 3, normalize=normalize)
+        if edit:
+            lab[over] = -1
+            w.masked_fill_(over, 0.0).mul_(2.0)
+        else:
+            lab, w = torch.where(over, -1, lab), torch.where(over, 0.0, w) * 2.0
+        res.append((w.detach(), lab, torch.autograd.grad(w, leaf, dw)[0]))
+    assert all(torch.equal(a, b) for a, b in zip(*res))
+
+
 # calls that are refused, on rows x [4, 8] and labels l [4] of either device
 REFUSALS = {
     "norm list": (lambda x, l: tdc.rms_norm([1.0]), TypeError),

@@ -140,6 +140,11 @@ def test_combine_never_looks_at_the_weight_of_a_dropped_slot(bad):
     rc.check_dropped_weights(torch.device("cpu"), bad)
 
 
+@pytest.mark.parametrize("normalize", [True, False])
+def test_gate_outputs_edited_in_place(normalize):
+    rc.check_gate_edited(torch.device("cpu"), normalize)
+
+
 # ----------------------------------------------------------------- refusals
 @pytest.mark.parametrize("name", rc.REFUSALS)
 def test_refusals(name):

@@ -239,6 +239,11 @@ def test_gate_nan_of_all_ones(gpu, clusters):
         assert not bool(w[0].isnan().any())
 
 
+@pytest.mark.parametrize("normalize", [True, False])
+def test_gate_outputs_edited_in_place(gpu, normalize):
+    rc.check_gate_edited(gpu, normalize)
+
+
 # ----------------------------------------------------------------- plan, group, combine
 @pytest.mark.parametrize("n,k,clusters", [(0, 2, 4), (1, 1, 1), (8, 2, 64), (4096, 1, 7), (4097, 1, 2047),
                                           (1500, 8, 256), (100, 1, 2048), (30000, 2, 65536),

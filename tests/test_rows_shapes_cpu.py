@@ -39,16 +39,17 @@ def gradients(x, r, w, y, wt, lab, mask):
     groups = tdc.group_plan(lab, 5)
     n, k = wt.shape
     stat = torch.zeros(n, 2, device=x.device)
-    chosen, labels = tdc.topk_gate(x, 3)
+    best, labels = tdc.topk_gate(x, 3)
+    chosen = torch.zeros(n, 3, 2, dtype=torch.int32, device=x.device)
     return [
         (ops.rms_norm_train(x, w, None, 1e-6), [x, torch.zeros(n, device=x.device)]),
         (ops.rms_norm_train(x, w, r, 1e-6), [x, x, torch.zeros(n, device=x.device)]),
         (ops.rms_norm_bwd(x, w, stat[:, 0].contiguous(), r, None, True), [x, w]),
         (ops.rms_norm_bwd(x, None, stat[:, 0].contiguous(), r, r, False), [x]),
-        (ops.topk_gate_train(x, None, 3, True), [chosen, labels]),
-        (ops.topk_gate_train(x, mask, 3, False), [chosen, labels, stat]),
-        ([ops.topk_gate_bwd(None, None, chosen, labels, None, chosen, 40, x.dtype)], [x]),
-        ([ops.topk_gate_bwd(x, mask, chosen, labels, stat, chosen, 40, x.dtype)], [x]),
+        (ops.topk_gate_train(x, None, 3, True), [best, labels, chosen]),
+        (ops.topk_gate_train(x, mask, 3, False), [best, labels, chosen, stat]),
+        ([ops.topk_gate_bwd(None, None, chosen, None, best, 40, x.dtype)], [x]),
+        ([ops.topk_gate_bwd(x, mask, chosen, stat, best, 40, x.dtype)], [x]),
         (ops.combine_rows_bwd(x, y, groups.offsets, groups.pos, wt, True), [y, wt]),
         (ops.combine_rows_bwd(x, None, groups.offsets, groups.pos, wt, True), [y]),
         (ops.combine_rows_bwd(x, y, groups.offsets, groups.pos, wt, False), [wt]),
