@@ -164,7 +164,8 @@ std::vector<Tensor> rms_norm_fp8(const Tensor& x, const OptTensor& w, const OptT
 }
 
 std::vector<Tensor> rms_norm_bwd(const Tensor& h, const OptTensor& w, const Tensor& rstd,
-                                 const Tensor& dy, const OptTensor& dh, bool want_dw) {
+                                 const Tensor& dy, const OptTensor& dh, bool want_dx,
+                                 bool want_dw) {
   check_rows(h, "h");
   check_like(dy, h, "dy");
   if (has(dh)) check_like(*dh, h, "dh");
@@ -175,12 +176,16 @@ std::vector<Tensor> rms_norm_bwd(const Tensor& h, const OptTensor& w, const Tens
   TORCH_CHECK(rstd.device() == h.device() && rstd.scalar_type() == at::kFloat &&
                   rstd.is_contiguous() && rstd.numel() == n, "tdc.rms_norm_bwd: rstd fp32 [N]");
   TORCH_CHECK(!want_dw || has(w), "tdc.rms_norm_bwd: dw needs the weights");
+  TORCH_CHECK(want_dx || (want_dw && !has(dh)), "tdc.rms_norm_bwd: nothing to compute, or dh without dx");
   bool w32;
   const void* wp = weights_of(w, w32);
   const DevGuard guard(h.device());
-  Tensor dx = fresh({n, d}, h.scalar_type(), h);
-  std::vector<Tensor> res = {dx};
-  Tensor part, dw;
+  std::vector<Tensor> res;
+  Tensor dx, part, dw;
+  if (want_dx) {
+    dx = fresh({n, d}, h.scalar_type(), h);
+    res.push_back(dx);
+  }
   const int parts = tdc_rms_norm_bwd_parts(n, num_cus(h));
   if (want_dw) {
     dw = fresh({d}, w->scalar_type(), *w);
@@ -189,7 +194,8 @@ std::vector<Tensor> rms_norm_bwd(const Tensor& h, const OptTensor& w, const Tens
   }
   check(tdc_rms_norm_bwd(code, h.data_ptr(), h.stride(0), rstd.data_ptr<float>(), wp, w32,
                          dy.data_ptr(), dy.stride(0), has(dh) ? dh->data_ptr() : nullptr,
-                         has(dh) ? dh->stride(0) : 0, n, (int)d, dx.data_ptr(),
+                         has(dh) ? dh->stride(0) : 0, n, (int)d,
+                         dx.defined() ? dx.data_ptr() : nullptr,
                          part.defined() ? part.data_ptr<float>() : nullptr, parts,
                          dw.defined() ? dw.data_ptr() : nullptr, cur_stream()),
         "rms_norm_bwd");
@@ -478,8 +484,10 @@ std::vector<Tensor> rms_norm_fp8_shapes(const Tensor& x, const OptTensor& w, con
   return norm_shapes(x, w, r, eps, false, width);
 }
 std::vector<Tensor> rms_norm_bwd_shapes(const Tensor& h, const OptTensor& w, const Tensor&,
-                                        const Tensor&, const OptTensor&, bool want_dw) {
-  std::vector<Tensor> res = {shaped(h.sym_sizes(), h.scalar_type(), h)};
+                                        const Tensor&, const OptTensor&, bool want_dx,
+                                        bool want_dw) {
+  std::vector<Tensor> res;
+  if (want_dx) res.push_back(shaped(h.sym_sizes(), h.scalar_type(), h));
   if (want_dw) res.push_back(shaped(w->sym_sizes(), w->scalar_type(), *w));
   return res;
 }
@@ -620,6 +628,10 @@ struct RmsNorm : public Function<RmsNorm> {
     ctx->set_materialize_grads(false);
     ctx->save_for_backward({has(r) ? out[1] : x, has(w) ? *w : Tensor(), rstd});
     ctx->saved_data["residual"] = has(r);
+    // without a gradient of the rows, their sum has none either
+    const bool rows = wants_grad(x) || wants_grad(r);
+    if (has(r) && !rows) ctx->mark_non_differentiable({out[1]});
+    ctx->saved_data["dx"] = rows;
     ctx->saved_data["dw"] = wants_grad(w);
     return out;
   }
@@ -627,6 +639,7 @@ struct RmsNorm : public Function<RmsNorm> {
     check_capture();
     const auto saved = ctx->get_saved_variables();
     const bool residual = ctx->saved_data["residual"].toBool();
+    const bool want_dx = ctx->saved_data["dx"].toBool();
     const bool want_dw = ctx->saved_data["dw"].toBool();
     const Tensor dh = grads.size() > 1 ? laid_out(grads[1]) : Tensor();
     variable_list res(4);
@@ -635,9 +648,9 @@ struct RmsNorm : public Function<RmsNorm> {
     } else {
       const std::vector<Tensor> g =
           TDC_BELOW_AUTOGRAD(rms_norm_bwd, saved[0], opt(saved[1]), saved[2], laid_out(grads[0]),
-                             opt(dh), want_dw);
-      res[0] = g[0];
-      if (want_dw) res[1] = g[1];
+                             opt(dh), want_dx, want_dw);
+      if (want_dx) res[0] = g[0];
+      if (want_dw) res[1] = g.back();
     }
     if (residual) res[2] = res[0];
     return once(res, grads, saved);
@@ -776,7 +789,8 @@ TORCH_LIBRARY_FRAGMENT(tdc, m) {
   m.def("combine_rows(Tensor y, Tensor offsets, Tensor pos, Tensor? w) -> Tensor");
   // the two halves of the autograd nodes
   m.def("rms_norm_train(Tensor x, Tensor? w, Tensor? r, float eps) -> Tensor[]");
-  m.def("rms_norm_bwd(Tensor h, Tensor? w, Tensor rstd, Tensor dy, Tensor? dh, bool want_dw) -> Tensor[]");
+  m.def("rms_norm_bwd(Tensor h, Tensor? w, Tensor rstd, Tensor dy, Tensor? dh, "
+        "bool want_dx, bool want_dw) -> Tensor[]");
   m.def("topk_gate_train(Tensor scores, Tensor? mask, int k, bool normalize) -> Tensor[]");
   m.def("topk_gate_bwd(Tensor? scores, Tensor? mask, Tensor chosen, Tensor? stat, Tensor dw, "
         "SymInt K, ScalarType dtype) -> Tensor");

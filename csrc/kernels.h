@@ -243,7 +243,8 @@ int tdc_quant_fp8(int src_dtype, const void* X, int64_t rows, int64_t valid, int
 int tdc_rms_norm(int dtype, const void* x, int64_t ldx, const void* r, int64_t ldr, const void* w,
                  int w32, int64_t n, int d, double eps, void* y, void* q, void* s, int dp, void* h,
                  float* rstd, hipStream_t stream);
-// dx [n, d] (+ dh, nullable) and, with dw, dw [d] through part fp32 [parts, d] scratch.
+// dx [n, d] (+ dh, nullable; dx null: not computed) and, with dw, dw [d] through part fp32
+// [parts, d] scratch.
 int tdc_rms_norm_bwd_parts(int64_t n, int cus);
 int tdc_rms_norm_bwd(int dtype, const void* h, int64_t ldh, const float* rstd, const void* w,
                      int w32, const void* dy, int64_t lddy, const void* dh, int64_t lddh,

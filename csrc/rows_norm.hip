@@ -216,6 +216,7 @@ __global__ __launch_bounds__(block_of<G>()) void norm_bwd_kernel(
         dot = fmaf(g[i][j], t[i][j], dot);
       }
     }
+    if (!dx) continue;  // dw alone is asked for
     const float c1 = group_sum<G>(dot, sums, turn) / (float)d;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {

@@ -1,5 +1,5 @@
 """Row operators under PyTorch's own machinery on the GPU: forward-mode gradients, dispatch
-modes, tracing, compilation."""
+modes, tracing, compilation, gradients that nobody asked for."""
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd
@@ -7,6 +7,7 @@ from torch.fx.experimental.proxy_tensor import make_fx
 from torch.utils._python_dispatch import TorchDispatchMode
 
 import tensorflow_distributed_clustering_amd as tdc
+from tests import rows_cases as rc
 
 pytestmark = pytest.mark.gpu
 
@@ -149,3 +150,20 @@ def test_registered_as_pytorch_asks(gpu):
                      (ops.combine_rows, (y, groups.offsets, groups.pos, v))):
         torch.library.opcheck(op.default, args, test_utils=(
             "test_schema", "test_autograd_registration", "test_faketensor", "test_aot_dispatch_dynamic"))
+
+
+@pytest.mark.parametrize("d", [7, 300, 5003])          # rows of a few threads, a wave, a block
+@pytest.mark.parametrize("with_sum", [False, True])
+def test_norm_with_a_gradient_of_the_weight_alone(gpu, d, with_sum):
+    x, r, dy = normal(gpu, 1, 70, d), normal(gpu, 2, 70, d), normal(gpu, 3, 70, d)
+    residual, w = (r if with_sum else None), normal(gpu, 4, d).requires_grad_()
+    out = tuple_of(tdc.rms_norm(x, w, residual=residual))
+    assert out[0].requires_grad and not any(h.requires_grad for h in out[1:])
+    with Seen() as seen:
+        dw, = torch.autograd.grad(out[0], w, dy)
+    assert len(seen.outs["rms_norm_bwd"]) == 1           # no gradient of rows is computed
+    h = rc.sum_kept(x, residual)
+    _, _, want, scale = rc.norm_grads(h, w.detach(), 1e-6, dy, None)
+    rc.close(dw, want, torch.float32, scale=scale, factor=2)
+    both, = torch.autograd.grad(tuple_of(tdc.rms_norm(x.requires_grad_(), w, residual=residual))[0], w, dy)
+    assert torch.equal(both, dw)

@@ -44,8 +44,9 @@ def gradients(x, r, w, y, wt, lab, mask):
     return [
         (ops.rms_norm_train(x, w, None, 1e-6), [x, torch.zeros(n, device=x.device)]),
         (ops.rms_norm_train(x, w, r, 1e-6), [x, x, torch.zeros(n, device=x.device)]),
-        (ops.rms_norm_bwd(x, w, stat[:, 0].contiguous(), r, None, True), [x, w]),
-        (ops.rms_norm_bwd(x, None, stat[:, 0].contiguous(), r, r, False), [x]),
+        (ops.rms_norm_bwd(x, w, stat[:, 0].contiguous(), r, None, True, True), [x, w]),
+        (ops.rms_norm_bwd(x, w, stat[:, 0].contiguous(), r, None, False, True), [w]),
+        (ops.rms_norm_bwd(x, None, stat[:, 0].contiguous(), r, r, True, False), [x]),
         (ops.topk_gate_train(x, None, 3, True), [best, labels, chosen]),
         (ops.topk_gate_train(x, mask, 3, False), [best, labels, chosen, stat]),
         ([ops.topk_gate_bwd(None, None, chosen, None, best, 40, x.dtype)], [x]),
