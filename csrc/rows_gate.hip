@@ -11,7 +11,7 @@
 //
 // Up to 8192 clusters a row stays in the registers of L threads, 8 to 32 scores each: as few
 // threads as hold it, since a round's part over the threads costs each of them the same (64M
-// bf16 scores, k = 8, in rows of 600: 54 us as 32 x 24, 78 as 64 x 16; in rows of 64: 60 us
+// bf16 scores, k = 8, in rows of 600: 57 us as 32 x 24, 78 as 64 x 16; in rows of 64: 60 us
 // as 8 x 8, 111 as 16 x 8).
 //
 // A score and its index become one number, the index in place of the score's last 6 to 13
@@ -21,7 +21,10 @@
 // is taken out.  Where fp32 loses bits that are not zero and two neighbours among the first
 // k + 1 choices agree in the bits that are left, the rows of that wave are chosen again by
 // the whole scores.  65536 x 256 fp32, k = 8: 21 us, 37 with whole scores in every round.
-// Bound by these instructions from k = 4 or so, by memory below.
+// With k = 1 it takes 13 us (5.3 TB/s), with k = 4 15: the rounds are what is added.  Vector
+// instructions fill 0.43, 0.55 and 0.59 of the issue slots at k = 1, 4 and 8, the cycles of
+// the launch itself counted in; 12289 x 1000 bf16, masked and over all, 20 us, 0.59 as well,
+// where a score is held twice.
 #include "rows_common.h"
 
 namespace tdc {
@@ -277,8 +280,9 @@ __global__ __launch_bounds__(GATE_BLOCK) void gate_kernel(const T* __restrict__ 
 
 // More clusters: a block per row takes 8192 scores at a time into its registers and their
 // best into a list of the k best so far, lane j of each wave holding the j-th: after the
-// first part few are better than its last.  65536 clusters, 1024 rows bf16, k = 8: 90 us, 840
-// with the row read again in every round.
+// first part few are better than its last.  65536 clusters, 1024 rows bf16, k = 8: 92 us (1.5
+// TB/s: a part is loaded when the one before it is done), 840 with the row read again in every
+// round.
 template <typename T, int TAIL, bool MASKED>
 __global__ __launch_bounds__(GATE_BLOCK) void gate_wide_kernel(
     const T* __restrict__ scores, int64_t ld, Mask mask, int64_t n, int K, int k, bool normalize,
@@ -372,7 +376,7 @@ __global__ __launch_bounds__(GATE_BLOCK) void gate_wide_kernel(
 // The gradient: L lanes per row, U vectors of each at a time.  What the chosen places get on
 // top of the rest goes through LDS, so that every place is stored once (a second store of
 // the chosen places would have to wait until the first have arrived).  65536 x 256 fp32:
-// 17.6 us, bound by its 67 MB of stores and the latency of the few loads before them.
+// 16 to 17 us, bound by its 67 MB of stores and the latency of the few loads before them.
 template <typename T, int L, int TAIL>
 __global__ __launch_bounds__(GATE_BLOCK) void gate_bwd_kernel(
     const T* __restrict__ scores, int64_t ld, Mask mask, const int2* __restrict__ chosen,

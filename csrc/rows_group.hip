@@ -235,8 +235,8 @@ __global__ __launch_bounds__(SORT_BLOCK) void sort_scatter_kernel(
 
 // The end of a sort in two passes.  pos[slot] holds the place after the first pass, `moved`
 // where the second put what stood there: the slot's place is read through both (1M labels:
-// 18 us for the second pass and 11 here; 31 and 5 where that pass wrote pos[slot] itself, 4
-// bytes at a time all over).  offsets[c] is the first place whose key is c or more, looked
+// 16 us for the second scatter and 11 here; 31 and 5 where it wrote pos[slot] itself, 4 bytes
+// at a time all over).  offsets[c] is the first place whose key is c or more, looked
 // up by halving among the places of its upper digit (`starts`): as long for clusters that
 // are all empty as for full ones.
 __global__ __launch_bounds__(SORT_BLOCK) void sort_finish_kernel(
@@ -323,8 +323,9 @@ __device__ __forceinline__ bool piece(int u, int L, int64_t n, int d, int pass, 
 
 // xg: every row is read once and written to the places of its k slots (zeros behind the
 // kept ones), J slots at a time: their places are all there before the first store, as a
-// wait for a load waits for the stores before it too (rows of 2 KiB with k = 8: 6.4 TB/s,
-// 3.5 with a place fetched before each store).
+// wait for a load waits for the stores before it too (rows of 2 KiB with k = 8, 302 MB: 47 us
+// through the caches, 86 with a place fetched before each store; 61 us, 5.0 TB/s, past the
+// caches, which pays in the next kernel).
 template <typename T, int J, int U, bool LONG, bool SHORT, bool STREAM>
 __global__ __launch_bounds__(256) void group_kernel(const T* __restrict__ x, int64_t ldx, int64_t n,
                                                     int k, int d, const int* __restrict__ offsets,
@@ -424,7 +425,7 @@ __global__ __launch_bounds__(256) void combine_kernel(const T* __restrict__ y, i
 
 // Gradients of a row's slots, J at a time: dy[p] = w dout[row], dw = <dout[row], y[p]>;
 // either may be left out (dy null, y null).  The row's passes and the sum over its lanes
-// are this thread group's, so dw needs no atomics.  131072 x 1024 bf16: 118 us, 4.8 TB/s
+// are this thread group's, so dw needs no atomics.  131072 x 1024 bf16: 120 us, 4.8 TB/s
 // (y, dout and dy once each).
 template <typename T, int J, int U, bool LONG, bool SHORT, bool STREAM>
 __global__ __launch_bounds__(256) void combine_bwd_kernel(
@@ -556,8 +557,9 @@ template <typename F> int with_slots(int k, F&& f) {
 
 struct SortShape {
   int low, high;  // bits of the first and the second pass's digit (0: one pass)
-  // slots per thread: one block sorts up to 4096 alone; from there enough chunks to fill the
-  // chip (1M labels, 65536 clusters: 63 us with 8, 66 with 16), then few enough counts
+  // slots per thread: one block sorts up to 2048 alone; from there enough chunks to fill the
+  // chip (1M labels, 65536 clusters: 63 us with 8, 66 with 16), then few enough counts (3M:
+  // 154 us)
   int per;
   int64_t chunks;
   int digits[2];

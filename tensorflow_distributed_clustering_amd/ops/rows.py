@@ -93,10 +93,11 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
     """``h / sqrt(mean(h^2) + eps) * weight`` of each row of ``h = x + residual``.
 
     Returns ``y``, or ``(y, h)`` with a residual.  ``h`` is rounded to the rows' type and
-    ``y`` is the norm of that rounded row, so ``h`` is all the gradient keeps.  ``weight``
-    [D] is fp32 or of the rows' type (None: ones).  The squares are summed in fp32: a row
-    whose sum of squares passes 3.4e38 becomes zeros.  With ``eps`` = 0 a row of zeros
-    becomes NaN."""
+    ``y`` is the norm of that rounded row, so ``h`` is all the gradient keeps (edited in place
+    before the gradient it raises).  ``weight`` [D] is fp32 or of the rows' type (None: ones).
+    The squares are summed in fp32: a row whose sum of squares passes 3.4e38 becomes zeros.
+    With ``eps`` = 0 a row of zeros becomes NaN, and one of values so small that their squares
+    are zeros in fp32 (below 1e-23) becomes infinite."""
     if not _on_gpu(x, weight, residual):
         _check_norm(x, weight, residual, eps)
         return ref.rms_norm(x, weight, residual, eps)
@@ -139,9 +140,9 @@ def fp8_width(d: int) -> int:
 
 def rms_norm_fp8(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
                  residual: Optional[torch.Tensor] = None, eps: float = 1e-6):
-    """:func:`rms_norm` whose ``y`` is computed in fp64 and rounded once to
-    :class:`Fp8Rows`, one exponent per 32 columns.  Returns the rows, or ``(rows, h)`` with a residual.  For
-    serving: it has no gradient, and refuses inputs that ask for one."""
+    """:func:`rms_norm` whose ``y`` is computed in fp64 and rounded to :class:`Fp8Rows`, one
+    exponent per 32 columns.  Returns the rows, or ``(rows, h)`` with a residual.  For serving:
+    it has no gradient, and refuses inputs that ask for one or have a forward-mode tangent."""
     gpu = _on_gpu(x, weight, residual)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
         raise RuntimeError("rms_norm_fp8 has no gradient: call it under torch.no_grad()")
