@@ -93,8 +93,8 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
     """``h / sqrt(mean(h^2) + eps) * weight`` of each row of ``h = x + residual``.
 
     Returns ``y``, or ``(y, h)`` with a residual.  ``h`` is rounded to the rows' type and
-    ``y`` is the norm of that rounded row, so ``h`` is all the gradient keeps (edited in place
-    before the gradient it raises).  ``weight`` [D] is fp32 or of the rows' type (None: ones).
+    ``y`` is the norm of that rounded row, so ``h`` is all the gradient keeps (on the
+    GPU the gradient raises where it was edited in place).  ``weight`` [D] is fp32 or of the rows' type (None: ones).
     The squares are summed in fp32: a row whose sum of squares passes 3.4e38 becomes zeros.
     With ``eps`` = 0 a row of zeros becomes NaN, and one of values so small that their squares
     are zeros in fp32 (below 1e-23) becomes infinite."""

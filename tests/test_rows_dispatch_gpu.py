@@ -1,10 +1,11 @@
 """Row operators under PyTorch's own machinery on the GPU: forward-mode gradients, dispatch
-modes, tracing, compilation, gradients that nobody asked for."""
+modes, tracing, compilation, checkpoints, function transforms, gradients that nobody asked for."""
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd
 from torch.fx.experimental.proxy_tensor import make_fx
 from torch.utils._python_dispatch import TorchDispatchMode
+from torch.utils.checkpoint import CheckpointPolicy, checkpoint, create_selective_checkpoint_contexts
 
 import tensorflow_distributed_clustering_amd as tdc
 from tests import rows_cases as rc
@@ -167,3 +168,53 @@ def test_norm_with_a_gradient_of_the_weight_alone(gpu, d, with_sum):
     rc.close(dw, want, torch.float32, scale=scale, factor=2)
     both, = torch.autograd.grad(tuple_of(tdc.rms_norm(x.requires_grad_(), w, residual=residual))[0], w, dy)
     assert torch.equal(both, dw)
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_checkpointed(gpu, name):
+    """Recomputed in the backward pass, whole and with the package's own results kept."""
+    call, _ = CALLS[name]
+    args = inputs(gpu, name)
+    want = with_grads(gpu, call, args)
+
+    def keep(ctx, op, *args, **kwargs):
+        return CheckpointPolicy.MUST_SAVE if op.namespace == "tdc" else CheckpointPolicy.PREFER_RECOMPUTE
+
+    for extra in ({}, {"context_fn": lambda: create_selective_checkpoint_contexts(keep)}):
+        again = lambda gpu, *a: checkpoint(lambda *b: tuple_of(call(gpu, *b)), *a, use_reentrant=False, **extra)  # noqa: E731,B023
+        assert all(torch.equal(a, b) for a, b in zip(with_grads(gpu, again, args), want))
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_function_transforms_are_right_or_refused(gpu, name):
+    call, _ = CALLS[name]
+    args = inputs(gpu, name)
+    first = lambda *a: tuple_of(call(gpu, *a))[0]  # noqa: E731
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda *a: first(*a).sum())(*args)
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(first, tuple(args), tuple(torch.ones_like(a) for a in args))
+    many = [torch.stack([a, 2 * a, -a]) for a in args]
+    if name.startswith("norm"):        # lists of results have no loop over a batch
+        with pytest.raises(RuntimeError):
+            torch.vmap(first)(*many)
+    else:
+        want = torch.stack([first(*(m[i] for m in many)) for i in range(3)])
+        assert torch.equal(torch.vmap(first)(*many), want)
+
+
+def test_gradients_of_leaves_are_their_own(gpu):
+    """x and residual have the same gradient, in memory of their own each."""
+    x, r = normal(gpu, 1, 6, 40).requires_grad_(), normal(gpu, 2, 6, 40).requires_grad_()
+    y, h = tdc.rms_norm(x, residual=r)
+    up = torch.ones_like(h)
+    torch.autograd.backward((y, h), (y.detach(), up))
+    kept = r.grad.clone()
+    assert torch.equal(x.grad, kept)
+    x.grad.zero_()
+    assert torch.equal(r.grad, kept) and bool((up == 1).all())
+    x.grad = None
+    y, h = tdc.rms_norm(x, residual=r.detach())
+    h.backward(up)                     # the incoming gradient goes through
+    x.grad.zero_()
+    assert bool((up == 1).all())
